@@ -21,6 +21,7 @@ NORM_BOX, NORM_L1, NORM_L2, NORM_INF = 0, 1, 2, 3
 OP_LINEAR, OP_CONV2D, OP_RELU, OP_FLATTEN = 1, 2, 3, 4
 REDUCE_MEAN, REDUCE_SUM, REDUCE_MIN, REDUCE_SOFTMIN = 0, 1, 2, 3
 OBJECTIVE_GAP, OBJECTIVE_BOTH = 2, 3
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 
 _p = C.c_void_p
 _i = C.c_int
@@ -123,6 +124,17 @@ SIGNATURES = {
     "bf_chain_alpha_shared_workspace_bytes": (_sz, [_p, _i, _i, _i]),
     "bf_chain_alpha_crown_shared": (_i, [_p] * 12 + [_i, _f, _p, _p, _p, _i, _f, _p, _sz, _i, _i, _p]),
     "bf_chain_alpha_beta_crown_shared_reduce": (_i, [_p] * 12 + [_i, _f, _p, _p, _p, _i, _f, _i, _f, _p, _sz, _i, _i, _p]),
+    "bf_w4_quantise": (_i, [_p, _i, _p, _p, _i, _i, _i, _p]),
+    "bf_w4_integers": (_i, [_p, _p, _i, _i, _i, _p]),
+    "bf_w4_dense": (_i, [_p, _p, _p, _i, _i, _i, _p]),
+    "bf_w4_linear": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _i, _p]),
+    "bf_w4_interval": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "bf_w4_rows": (_i, [_p, _i, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "bf_w4_interval_grad": (_i, [_p] * 6 + [_i] * 4 + [_p]),
+    "bf_rows_dot": (_i, [_p, _p, _p, _i, _i, _i, _p]),
+    "bf_column_sums": (_i, [_p, _i, _p, _i, _i, _i, _p]),
+    "bf_adamw_step": (_i, [_p, _i, _i, _i, _i, _p, _p, _p, _p, C.c_double, C.c_double, _f, _p, _p, _i, _p]),
+    "bf_adamw_moments": (_i, [_p] * 6 + [C.c_longlong, _p]),
 }
 
 _lib: Optional[C.CDLL] = None

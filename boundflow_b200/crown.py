@@ -29,7 +29,8 @@ import torch
 
 from . import _lib
 from .ir import IntervalState, input_mid_rad, lp_ball_of, normalize_input_spec
-from .network import CudaChain, compile_chain
+from .network import CudaChain, _cuda_device, _f32, _stream_ptr, compile_chain
+from .weights4 import Weight4
 
 
 @dataclass
@@ -72,23 +73,6 @@ class CrownIbpStats:
     supported: bool
     reason: str = ""
     ops_seen: Tuple[str, ...] = ()
-
-
-def _cuda_device(t: torch.Tensor) -> torch.device:
-    if t.device.type == "cuda":
-        return t.device
-    if not torch.cuda.is_available():
-        raise RuntimeError("boundflow_b200 needs a CUDA device (no CPU fallback exists)")
-    return torch.device("cuda", torch.cuda.current_device())
-
-
-def _f32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    return t.detach().to(device=device, dtype=torch.float32, non_blocking=True).contiguous()
-
-
-def _stream_ptr(device: torch.device) -> int:
-    """Handle of the current stream (`torch.cuda.current_stream(device).cuda_stream` without the Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 class _Workspace:
@@ -498,11 +482,14 @@ def crown_from_trace(
 
 def needs_graph_path(module: Any) -> bool:
     """True when the entry task is not a chain: an op merges values (add, concat) or does not consume
-    the previous op's output (fan-out, skip connections)."""
+    the previous op's output (fan-out, skip connections); and for chains with a 4-bit weight, which the fused sweeps do not read."""
     task = module.get_entry_task()
+    params = module.bindings.get("params", {})
     cur = task.input_values[0] if task.input_values else None
     for op in task.ops:
         if op.op_type in ("add", "concat") or not op.inputs or op.inputs[0] != cur:
+            return True
+        if op.op_type == "linear" and isinstance(params, dict) and isinstance(params.get(op.inputs[1]), Weight4):
             return True
         cur = op.outputs[0]
     return False

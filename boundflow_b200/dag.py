@@ -21,10 +21,11 @@ from typing import Any, Dict, List, Mapping, Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, weights4
 from .crown import _alpha_rows, _cuda_device, _f32, _split_tensor, _stream_ptr, relax_all
 from .ir import IntervalState, input_mid_rad, lp_ball_of, normalize_input_spec
 from .network import dense_conv_weight
+from .weights4 import Weight4
 
 
 def _numel(shape) -> int:
@@ -63,15 +64,20 @@ class DagTrace:
 
 
 def _params(module: Any, device: torch.device) -> Dict[str, torch.Tensor]:
-    """Parameters as fp32 device tensors; the weight of a grouped or dilated Conv2d op is replaced by its dense
+    """Parameters as fp32 device tensors, 4-bit weights as they are; the weight of a grouped or dilated Conv2d op is replaced by its dense
     equivalent (`network.dense_conv_weight`), so every step of the walkers sees groups = 1, dilation = 1."""
     raw = module.bindings.get("params", {})
     out = {}
     for k, v in (raw.items() if isinstance(raw, dict) else []):
+        if isinstance(v, Weight4):
+            out[k] = v.to(device)
+            continue
         t = v if torch.is_tensor(v) else torch.as_tensor(v)
         out[k] = _f32(t, device)
     dense_for: Dict[str, Tuple[int, Tuple[int, int]]] = {}
     for op in module.get_entry_task().ops:
+        if op.op_type != "linear" and any(isinstance(out.get(nm), Weight4) for nm in op.inputs):
+            raise NotImplementedError(f"{op.op_type} '{op.name}': only Linear layers take a 4-bit weight")
         if op.op_type != "conv2d" or len(op.inputs) < 2 or op.inputs[1] not in out:
             continue
         key = (int(op.attrs.get("groups", 1)), _pair(op.attrs.get("dilation", 1)))
@@ -124,7 +130,12 @@ def forward_ibp_dag(module: Any, input_spec: Any, relu_split_state: Optional[Map
                 if _numel(tr.shape[x]) != n_in:
                     raise ValueError(f"linear '{op.name}': weight {tuple(W.shape)} does not match input shape {tr.shape[x]}")
                 yl, yu = torch.empty(B, n_out, device=device), torch.empty(B, n_out, device=device)
-                if at_input and ball is not None:
+                if isinstance(W, Weight4) and at_input and ball is not None:
+                    W = W.dense()  # the dual norms of its rows are taken of what the codes stand for
+                if isinstance(W, Weight4):
+                    a, bb, mode = (tr.mid, tr.rad, _lib.IN_MID_RAD) if at_input else (tr.lower[x], tr.upper[x], _lib.IN_LOWER_UPPER)
+                    yl, yu = weights4._interval(a.contiguous(), bb.contiguous(), mode, 0, W, b)
+                elif at_input and ball is not None:
                     row_dev = torch.empty(n_out, dtype=torch.float32, device=device)
                     _lib.check(lib.bf_row_dual_norms(_lib.ptr(W), n_out, n_in, tr.norm_p, tr.eps, _lib.ptr(row_dev), s))
                     _lib.check(lib.bf_ibp_linear_lp(_lib.ptr(tr.mid), _lib.ptr(row_dev), _lib.ptr(W), _lib.ptr(b), None, 0, None, None,
@@ -259,7 +270,8 @@ def _sides_join(module: Any, tr: DagTrace, params: Dict[str, torch.Tensor], S: i
     rows = 2 * tr.B * S
     if len(tr.shape[output_value]) == 3 or rows * max(_numel(sh) for sh in tr.shape.values()) * 4 > 1 << 30:
         return False
-    return rows < 256 or all(op.op_type != "linear" or min(params[op.inputs[1]].shape) < 32 for op in module.get_entry_task().ops)
+    return rows < 256 or all(op.op_type != "linear" or isinstance(params[op.inputs[1]], Weight4) or min(params[op.inputs[1]].shape) < 32
+                             for op in module.get_entry_task().ops)
 
 
 def _sweep(lib, module: Any, tr: DagTrace, params: Dict[str, torch.Tensor], relax, C: torch.Tensor, side: int, output_value: str, *,
@@ -303,6 +315,12 @@ def _sweep(lib, module: Any, tr: DagTrace, params: Dict[str, torch.Tensor], rela
             W = params[op.inputs[1]]
             b = params[op.inputs[2]] if len(op.inputs) == 3 else None
             n_cur, n_prev = int(W.shape[0]), int(W.shape[1])
+            if isinstance(W, Weight4):
+                rows = st.A.reshape(B * S, n_cur)
+                if b is not None:
+                    _lib.check(lib.bf_rows_dot(_lib.ptr(rows), _lib.ptr(b), _lib.ptr(st.d), 1, B * S, n_cur, s))
+                push(op.inputs[0], weights4._rows(rows, W).view(B, S, n_prev), st.d)
+                continue
             Ap = torch.empty(B, S, n_prev, device=device)
             pack = _lib.LINEAR_PACKS.get(W, B * S, s)  # tensor-core path for large coefficient blocks
             _lib.check(lib.bf_crown_relu_linear_bwd_packed(_lib.ptr(st.A), side, None, None, None, None, None, _lib.ptr(W), _lib.ptr(b),
@@ -468,6 +486,9 @@ def _adjoint_forward(lib, module: Any, tr: DagTrace, params: Dict[str, torch.Ten
             W = params[op.inputs[1]]
             b = params[op.inputs[2]] if len(op.inputs) == 3 else None
             n_out, n_in = int(W.shape[0]), int(W.shape[1])
+            if isinstance(W, Weight4):
+                h[out] = weights4._linear(h[x].reshape(B * S, n_in), W, b).view(B, S, n_out)
+                continue
             Wt = _TRANSPOSED.get(W)
             g = torch.empty(B, S, n_out, device=device)
             # rows x W^T: the backward entry point on the transposed weight, no slopes, no bias term
@@ -739,6 +760,7 @@ def first_layer_certificate_dag(module: Any, input_spec: Any, relu_split_state: 
         if raw is None or prod is None or prod.op_type not in ("linear", "conv2d") or not prod.inputs or prod.inputs[0] != spec.value_name:
             continue
         W = params[prod.inputs[1]]
+        W = W.dense() if isinstance(W, Weight4) else W
         b = params[prod.inputs[2]] if len(prod.inputs) == 3 else None
         if prod.op_type == "linear":
             n1 = int(W.shape[0])

@@ -21,6 +21,7 @@ from . import _lib
 from .crown import _cuda_device, _f32, _plain_set, _stream_ptr, ibp_query, ibp_trace, needs_graph_path
 from .ir import IntervalState, input_mid_rad, lp_ball_of, normalize_input_spec
 from .network import _pair, compile_chain, dense_conv_weight
+from .weights4 import Weight4, interval_linear4
 
 
 def _is_interval_kind(kind: Any) -> bool:
@@ -52,6 +53,12 @@ class CudaIntervalDomain:
         lib = _lib.load()
         x_l, x_u = state_in.lower, state_in.upper
         device = _cuda_device(x_l)
+        if isinstance(weight, Weight4):
+            if attrs.get("op") not in (None, "linear"):
+                raise NotImplementedError(f"{attrs.get('op')}: only Linear layers take a 4-bit weight")
+            b4 = None if bias is None else _f32(bias if torch.is_tensor(bias) else torch.as_tensor(bias), device)
+            y_l, y_u = interval_linear4(_f32(x_l, device), _f32(x_u, device), weight, b4, relu_in=bool(attrs.get("relu_in", False)))
+            return _state_like(state_in, y_l.to(x_l.device), y_u.to(x_l.device))
         w = weight if torch.is_tensor(weight) else torch.as_tensor(weight)
         w = _f32(w, device)
         b = None
@@ -306,7 +313,8 @@ class CudaTaskExecutor:
             if ball is None or op.inputs[0] not in views:
                 return None
             lib = _lib.load()
-            W = _f32(get_tensor(op.inputs[1]), device)
+            W = get_tensor(op.inputs[1])
+            W = W.to(device).dense() if isinstance(W, Weight4) else _f32(W, device)
             if W.dim() != 2:
                 return None
             b = _f32(get_tensor(op.inputs[2]), device) if len(op.inputs) == 3 else None

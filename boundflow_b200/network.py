@@ -21,6 +21,23 @@ import torch
 from . import _lib
 
 
+def _cuda_device(t: torch.Tensor) -> torch.device:
+    if t.device.type == "cuda":
+        return t.device
+    if not torch.cuda.is_available():
+        raise RuntimeError("boundflow_b200 needs a CUDA device (no CPU fallback exists)")
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def _f32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    return t.detach().to(device=device, dtype=torch.float32, non_blocking=True).contiguous()
+
+
+def _stream_ptr(device: torch.device) -> int:
+    """Handle of the current stream (`torch.cuda.current_stream(device).cuda_stream` without the Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
 def _pair(v: Any) -> Tuple[int, int]:
     if isinstance(v, int):
         return (int(v), int(v))
@@ -113,6 +130,8 @@ class CudaChain:
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise RuntimeError("the B200 backend needs a CUDA device; there is no CPU path")
+        from .weights4 import Weight4  # (which takes its helpers from here)
+
         task = module.get_entry_task()
         if getattr(module, "task_graph", None) is not None or len(module.tasks) != 1:
             raise NotImplementedError("chain compilation supports single-task modules only")
@@ -127,6 +146,8 @@ class CudaChain:
 
         def dev(name: str, attrs: Any = None) -> torch.Tensor:
             t = params[name]
+            if isinstance(t, Weight4):
+                raise NotImplementedError(f"'{name}' is held in 4 bits: the fused sweeps read dense weights (the functions of crown.py and dag.py take it)")
             given = t if torch.is_tensor(t) else torch.as_tensor(t)
             out = dense_conv_weight(given.detach().to(device=self.device, dtype=torch.float32).contiguous(), attrs)
             if torch.is_tensor(t) and out.data_ptr() != t.data_ptr():

@@ -1,0 +1,272 @@
+"""Linear layers whose weights are held in 4 bits with a scale for each group of columns.
+
+`Weight4` stands where a Linear layer's weight does: in the `params` of a module that `CudaTaskExecutor.run_ibp`, `run_crown_ibp_mlp`,
+`run_alpha_beta_crown_mlp` and the other whole-query functions bound (such modules take the graph path of `dag.py`), as the weight of
+`CudaIntervalDomain.affine_transformer`, and in the products below:
+
+    linear4(x, weight, bias)                   x W^T + b, with gradients for x and bias (the weight is frozen)
+    interval_linear4(lower, upper, weight, b)  bounds of it over boxes, with gradients for lower, upper and bias
+    rows_times_weight4(A, weight)              A W: coefficient rows pushed back through the layer
+    quantise_weight4(W, group)                 codes and scales of a given weight
+
+The reference holds all weights in 32 bits; the bounds are those of the network whose weights the codes and scales stand for, computed as
+`bf_ibp_linear` and `bf_crown_relu_linear_bwd` compute them for dense weights.  Like the rest of the package the functions queue their work on the current
+stream of the tensors' device; tensors on the CPU are copied to the current CUDA device and results returned on the device the inputs came from.
+"""
+from __future__ import annotations
+
+from typing import Any, Optional, Tuple
+
+import torch
+
+from . import _lib
+from .network import _cuda_device, _stream_ptr
+
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
+
+
+class Weight4:
+    """W [n_out, n_in] = scales[k // group, n] * (code[n, k] - 8).
+
+    codes: uint8 [n_out, padded / 2], two codes in a byte (low nibble = even column), padded = n_in rounded up to a whole group;
+    scales: fp32 [padded / group, n_out], finite.  Both contiguous, on one device, codes on a 16-byte boundary.  They are read where they are: a change
+    in place is a change of the weight."""
+
+    __slots__ = ("codes", "scales", "n_out", "n_in", "group")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n_in: int):
+        n_in = int(n_in)
+        if not (torch.is_tensor(codes) and torch.is_tensor(scales)) or codes.dtype != torch.uint8 or scales.dtype != torch.float32:
+            raise TypeError("Weight4 takes codes as uint8 and scales as float32 tensors")
+        if codes.dim() != 2 or scales.dim() != 2 or n_in < 1 or codes.shape[0] < 1:
+            raise ValueError(f"Weight4: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, n_in {n_in}")
+        n_out, padded, groups = int(codes.shape[0]), 2 * int(codes.shape[1]), int(scales.shape[0])
+        group = padded // groups if groups else 0
+        if int(scales.shape[1]) != n_out or groups == 0 or group * groups != padded or not padded - group < n_in <= padded:
+            raise ValueError(f"Weight4: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {n_in} weights")
+        if group < 32 or group > 1 << 20 or group & (group - 1):
+            raise ValueError(f"Weight4: groups of {group} weights (a power of two from 32 to 2^20 is wanted)")
+        if codes.device != scales.device:
+            raise ValueError("Weight4: codes and scales are on different devices")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
+            raise ValueError("Weight4: codes and scales must be contiguous, codes on a 16-byte boundary")
+        self.codes, self.scales, self.n_out, self.n_in, self.group = codes, scales, n_out, n_in, group
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.n_out, self.n_in)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dim(self) -> int:
+        return 2
+
+    def to(self, device: Any) -> "Weight4":
+        device = torch.device(device)
+        return self if device == self.device else Weight4(self.codes.to(device), self.scales.to(device), self.n_in)
+
+    def integers(self) -> torch.Tensor:
+        """code - 8 as int8 [n_out, n_in]."""
+        device = _device_of(self.codes)
+        w = self.to(device)
+        out = torch.empty(w.shape, dtype=torch.int8, device=device)
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().bf_w4_integers(w.codes.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group, _stream_ptr(device)))
+        return out.to(self.device)
+
+    def dense(self) -> torch.Tensor:
+        """The weight in fp32."""
+        device = _device_of(self.codes)
+        w = self.to(device)
+        out = torch.empty(w.shape, dtype=torch.float32, device=device)
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().bf_w4_dense(w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group, _stream_ptr(device)))
+        return out.to(self.device)
+
+    def __repr__(self) -> str:
+        return f"Weight4({self.n_out} x {self.n_in}, groups of {self.group}, {self.device})"
+
+
+def _device_of(t: torch.Tensor) -> torch.device:
+    return t.device if t.is_cuda else _cuda_device(t)
+
+
+def quantise_weight4(W: torch.Tensor, group: int = 128) -> Weight4:
+    """Codes and scales of W (fp32, bf16 or fp16, [n_out, n_in]): the scale of a group is its largest magnitude times 1/7, a code the nearest of -7..7
+    (ties to even).  A group of zeros has scale 0; one that holds an infinity or a NaN is NaN throughout."""
+    if not torch.is_tensor(W) or W.dtype not in _TYPES:
+        raise TypeError("quantise_weight4 takes an fp32, bf16 or fp16 tensor")
+    group = int(group)
+    if W.dim() != 2 or W.shape[0] < 1 or W.shape[1] < 1:
+        raise ValueError(f"quantise_weight4: a weight [n_out, n_in] is wanted, got {tuple(W.shape)}")
+    if group < 32 or group > 1 << 20 or group & (group - 1):
+        raise ValueError(f"quantise_weight4: groups of {group} weights (a power of two from 32 to 2^20 is wanted)")
+    device = _device_of(W)
+    w = W.detach().to(device).contiguous()
+    n_out, n_in = int(w.shape[0]), int(w.shape[1])
+    groups = -(-n_in // group)
+    codes = torch.empty(n_out, groups * group // 2, dtype=torch.uint8, device=device)
+    scales = torch.empty(groups, n_out, dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().bf_w4_quantise(w.data_ptr(), _TYPES[w.dtype], codes.data_ptr(), scales.data_ptr(), n_out, n_in, group, _stream_ptr(device)))
+    return Weight4(codes, scales, n_in).to(W.device)
+
+
+# ---- launches: contiguous CUDA tensors of one device, rows [M, n] -----------------------
+def _linear(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    M, device = int(x.shape[0]), x.device
+    y = torch.empty(M, w.n_out, dtype=x.dtype, device=device)
+    if M:
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().bf_w4_linear(x.data_ptr(), _TYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), _lib.ptr(bias),
+                                                _TYPES[bias.dtype] if bias is not None else 0, y.data_ptr(), M, w.n_in, w.n_out, w.group, _stream_ptr(device)))
+    return y
+
+
+def _interval(a: torch.Tensor, b: torch.Tensor, mode: int, relu_in: int, w: Weight4, bias: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    M, device = int(a.shape[0]), a.device
+    lower, upper = (torch.empty(M, w.n_out, dtype=torch.float32, device=device) for _ in range(2))
+    if M:
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().bf_w4_interval(a.data_ptr(), b.data_ptr(), mode, relu_in, w.codes.data_ptr(), w.scales.data_ptr(), _lib.ptr(bias), lower.data_ptr(),
+                                                  upper.data_ptr(), M, w.n_in, w.n_out, w.group, _stream_ptr(device)))
+    return lower, upper
+
+
+def _rows(a: torch.Tensor, w: Weight4) -> torch.Tensor:
+    M, device = int(a.shape[0]), a.device
+    z = torch.empty(M, w.n_in, dtype=a.dtype, device=device)
+    if M:
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().bf_w4_rows(a.data_ptr(), _TYPES[a.dtype], w.codes.data_ptr(), w.scales.data_ptr(), z.data_ptr(), M, w.n_in, w.n_out, w.group,
+                                              _stream_ptr(device)))
+    return z
+
+
+def _column_sums(a: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    M, n, device = int(a.shape[0]), int(a.shape[1]), a.device
+    if M == 0:
+        return torch.zeros(n, dtype=dtype, device=device)
+    out = torch.empty(n, dtype=dtype, device=device)
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().bf_column_sums(a.data_ptr(), _TYPES[a.dtype], out.data_ptr(), _TYPES[dtype], M, n, _stream_ptr(device)))
+    return out
+
+
+class _Linear4(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, weight):
+        ctx.weight, ctx.bias_type = weight, None if bias is None else bias.dtype
+        return _linear(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dy = dy.contiguous()
+        dx = _rows(dy, ctx.weight) if ctx.needs_input_grad[0] else None
+        db = _column_sums(dy, ctx.bias_type) if ctx.needs_input_grad[1] else None
+        return dx, db, None
+
+
+class _Interval4(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lower, upper, bias, weight):
+        ctx.weight = weight
+        return _interval(lower, upper, _lib.IN_LOWER_UPPER, 0, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dl, du):
+        w, device = ctx.weight, dl.device
+        dl, du = dl.contiguous(), du.contiguous()
+        M = int(dl.shape[0])
+        gl = gu = db = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            gl, gu = (torch.empty(M, w.n_in, dtype=torch.float32, device=device) for _ in range(2))
+            if M:
+                with torch.cuda.device(device):
+                    _lib.check(_lib.load().bf_w4_interval_grad(dl.data_ptr(), du.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gl.data_ptr(), gu.data_ptr(),
+                                                               M, w.n_in, w.n_out, w.group, _stream_ptr(device)))
+        if ctx.needs_input_grad[2]:
+            db = _column_sums(dl, torch.float32) + _column_sums(du, torch.float32)
+        return gl, gu, db, None
+
+
+def _check_rows(name: str, x: Any, weight: Any, width: str) -> None:
+    if not isinstance(weight, Weight4):
+        raise TypeError(f"{name}: the weight is a Weight4 (quantise_weight4 makes one), got {type(weight)}")
+    if not torch.is_tensor(x) or x.dtype not in _TYPES:
+        raise TypeError(f"{name} takes fp32, bf16 or fp16 tensors")
+    if x.dim() < 1 or int(x.shape[-1]) != getattr(weight, width):
+        raise ValueError(f"{name}: rows of {int(x.shape[-1]) if x.dim() else 0} do not match {weight!r}")
+
+
+def _check_bias(name: str, bias: Any, weight: Weight4) -> None:
+    if bias is not None and (not torch.is_tensor(bias) or bias.dtype not in _TYPES):
+        raise TypeError(f"{name} takes an fp32, bf16 or fp16 bias")
+    if bias is not None and tuple(bias.shape) != (weight.n_out,):
+        raise ValueError(f"{name}: bias {tuple(bias.shape)} does not match {weight!r}")
+
+
+def _at(t: Optional[torch.Tensor], device: torch.device) -> Optional[torch.Tensor]:
+    return t if t is None or t.device == device else t.to(device)
+
+
+def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable once, for x and bias."""
+    _check_rows("linear4", x, weight, "n_in")
+    _check_bias("linear4", bias, weight)
+    device = _device_of(x)
+    w, b = weight.to(device), _at(bias, device)
+    rows = _at(x, device).reshape(-1, weight.n_in).contiguous()
+    if b is not None:
+        b = b.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        y = _Linear4.apply(rows, b, w)
+    else:
+        y = _linear(rows, w, b)
+    if x.dim() != 2:
+        y = y.reshape(x.shape[:-1] + (weight.n_out,))
+    return y if y.device == x.device else y.to(x.device)
+
+
+def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None, *,
+                     relu_in: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Bounds of x W^T + bias for lower <= x <= upper (fp32 [..., n_in]); `relu_in` clamps the input at zero first.  Differentiable once, for lower, upper
+    and bias (without relu_in)."""
+    _check_rows("interval_linear4", lower, weight, "n_in")
+    _check_rows("interval_linear4", upper, weight, "n_in")
+    _check_bias("interval_linear4", bias, weight)
+    if lower.shape != upper.shape or lower.device != upper.device:
+        raise ValueError(f"interval_linear4: lower {tuple(lower.shape)} and upper {tuple(upper.shape)} differ in shape or device")
+    if lower.dtype != torch.float32 or upper.dtype != torch.float32 or (bias is not None and bias.dtype != torch.float32):
+        raise TypeError("interval_linear4 takes fp32: bounds rounded to 16 bits would not hold")
+    device = _device_of(lower)
+    w, b = weight.to(device), _at(bias, device)
+    lo, up = (_at(t, device).reshape(-1, weight.n_in).contiguous() for t in (lower, upper))
+    if b is not None:
+        b = b.contiguous()
+    if torch.is_grad_enabled() and (lower.requires_grad or upper.requires_grad or (bias is not None and bias.requires_grad)):
+        if relu_in:
+            raise NotImplementedError("interval_linear4 has no gradient with relu_in; clamp the bounds before the call")
+        yl, yu = _Interval4.apply(lo, up, b, w)
+    else:
+        yl, yu = _interval(lo, up, _lib.IN_LOWER_UPPER, 1 if relu_in else 0, w, b)
+    if lower.dim() != 2:
+        shape = lower.shape[:-1] + (weight.n_out,)
+        yl, yu = yl.reshape(shape), yu.reshape(shape)
+    return (yl, yu) if yl.device == lower.device else (yl.to(lower.device), yu.to(lower.device))
+
+
+def rows_times_weight4(A: torch.Tensor, weight: Weight4) -> torch.Tensor:
+    """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once).  No gradient: it is one, of `linear4`."""
+    _check_rows("rows_times_weight4", A, weight, "n_out")
+    if torch.is_grad_enabled() and A.requires_grad:
+        raise NotImplementedError("rows_times_weight4 has no gradient; detach the rows")
+    device = _device_of(A)
+    z = _rows(_at(A, device).reshape(-1, weight.n_out).contiguous(), weight.to(device))
+    if A.dim() != 2:
+        z = z.reshape(A.shape[:-1] + (weight.n_in,))
+    return z if z.device == A.device else z.to(A.device)

@@ -705,6 +705,64 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
                                             int steps, float lr, int spec_reduce, float soft_tau,
                                             void* workspace, size_t workspace_bytes, int B, int S, bf_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Linear layers with 4-bit weights, and AdamW over many tensors (the reference has neither; they stand beside bf_ibp_linear,
+ * bf_crown_relu_linear_bwd and the Adam steps above)
+ * ---------------------------------------------------------------------- */
+
+#define BF_TYPE_F32 0
+#define BF_TYPE_BF16 1
+#define BF_TYPE_F16 2
+
+/* A 4-bit weight W [n_out, n_in]: W[n,k] = scales[k / group, n] * (code[n,k] - 8) with codes 0..15, two in a byte (low nibble = even
+ * column), rows of padded / 2 bytes where padded is n_in rounded up to a whole group (what the padding holds has no effect); scales fp32
+ * [padded / group, n_out], finite; group a power of two from 32 to 2^20; codes on a 16-byte boundary.  M rows, contiguous.
+ *   bf_w4_quantise       codes and scales of W (fp32 / bf16 / fp16): scale = max |w| of the group times 1/7 (as a 32-bit number), code = w / scale to the nearest (ties to
+ *                        even) + 8; a group of zeros has scale 0, one with an infinity or a NaN is NaN throughout.
+ *   bf_w4_integers       code - 8 as int8 [n_out, n_in];  bf_w4_dense: W as fp32 [n_out, n_in].
+ *   bf_w4_linear         y [M,n_out] = x [M,n_in] W^T + bias (or NULL); x and y of `type`, sums in fp32.
+ *   bf_w4_interval       bounds of the same over boxes, as bf_ibp_linear computes them: W c + b -/+ |W| r; in_mode BF_IN_LOWER_UPPER or
+ *                        BF_IN_MID_RAD, relu_in (with BF_IN_LOWER_UPPER) clamps the input at zero first.
+ *   bf_w4_rows           z [M,n_in] = a [M,n_out] W: coefficient rows pushed back through the layer, or the gradient of bf_w4_linear.
+ *   bf_w4_interval_grad  gradients of bf_w4_interval (BF_IN_LOWER_UPPER, no relu_in) for those of its two results.
+ * A sum over the codes of one group is scaled when it is complete: products of 2^124 / group and more overflow.
+ *   bf_rows_dot          d [M] = (accumulate: +=) A [M,n] . bias [n]: the bias term of a coefficient row.
+ *   bf_column_sums       out [n] = sum over the M rows of A, in order: the gradient of a bias. */
+int bf_w4_quantise(const void* W, int type, uint8_t* codes, float* scales, int n_out, int n_in, int group, bf_stream_t stream);
+int bf_w4_integers(const uint8_t* codes, int8_t* out, int n_out, int n_in, int group, bf_stream_t stream);
+int bf_w4_dense(const uint8_t* codes, const float* scales, float* out, int n_out, int n_in, int group, bf_stream_t stream);
+int bf_w4_linear(const void* x, int type, const uint8_t* codes, const float* scales, const void* bias, int bias_type, void* y, int M, int n_in,
+                 int n_out, int group, bf_stream_t stream);
+int bf_w4_interval(const float* in_a, const float* in_b, int in_mode, int relu_in, const uint8_t* codes, const float* scales, const float* bias,
+                   float* out_l, float* out_u, int M, int n_in, int n_out, int group, bf_stream_t stream);
+int bf_w4_rows(const void* a, int type, const uint8_t* codes, const float* scales, void* z, int M, int n_in, int n_out, int group,
+               bf_stream_t stream);
+int bf_w4_interval_grad(const float* grad_l, const float* grad_u, const uint8_t* codes, const float* scales, float* z_l, float* z_u, int M, int n_in,
+                        int n_out, int group, bf_stream_t stream);
+int bf_rows_dot(const float* A, const float* bias, float* d, int accumulate, int M, int n, bf_stream_t stream);
+int bf_column_sums(const void* A, int type, void* out, int out_type, int M, int n, bf_stream_t stream);
+
+/* One tensor of an AdamW step (HOST struct; p and g are device pointers).  `first`: where its moments begin in the flat buffers, a multiple of 256. */
+typedef struct {
+  void* p;
+  const void* g;
+  long long n;
+  long long first;
+  float lr, weight_decay;
+} bf_adamw_tensor;
+
+/* One AdamW step (decoupled weight decay) over `count` tensors (HOST array) of one type:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * with g multiplied by grad_scale[0] (device fp32, or NULL) first.  Gradients have the parameters' type, or any of the three beside fp32 parameters.
+ * m, v: flat moments on 16-byte boundaries, fp32 (state_bits 32), or one byte an element (8) with m_exponent, v_exponent, a byte for each 256 elements.
+ * state: 4 doubles on the device, beta1^t, beta2^t, t, 0, before the first step 1, 1, 0, 0; the call with `last` set moves it on when it is done, so that
+ * calls for several types or groups make one step, and a captured step counts as it is replayed.  count 0 with `last` only counts.
+ *   bf_adamw_moments  the values that 8-bit moments stand for, as bf16 [n] (exact); n a multiple of 256. */
+int bf_adamw_step(const bf_adamw_tensor* tensors, int count, int p_type, int g_type, int state_bits, void* m, void* v, uint8_t* m_exponent,
+                  uint8_t* v_exponent, double beta1, double beta2, float eps, const float* grad_scale, double* state, int last, bf_stream_t stream);
+int bf_adamw_moments(const uint8_t* m, const uint8_t* v, const uint8_t* m_exponent, const uint8_t* v_exponent, void* m_out, void* v_out, long long n,
+                     bf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
