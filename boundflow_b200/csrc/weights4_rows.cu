@@ -1,0 +1,271 @@
+// z = a W for few rows a and 4-bit weights, and the gradients of interval bounds (W and |W|); weights4_mma.cuh says how.
+#include "weights4_mma.cuh"
+
+namespace bf {
+namespace {
+
+// A block takes 128 columns and (with its cluster) splits the outputs over its warps, 32 at a time.  The scale belongs to the sum's index here, so it goes
+// into the rows: a[m, n] * scale[group, n], rounded to 32 bits and split into parts, by each warp for the outputs it reads.
+// Columns are the instruction's rows: lane (g, t) takes half a word (four columns) of each of the outputs 2t, 2t + 1, 2t + 8, 2t + 9.
+// P parts of a row, side by side (PACKED, one tile) or an instruction each for NT tiles of 8 rows; STEPS of 32 columns share a scale (1, 2, or 4 and more).
+template <int P, bool PACKED, int NT, bool DUAL, int STEPS>
+__global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p, const Split sp) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int Q = PACKED ? 1 : P * NT, SETS = DUAL ? 2 : 1;
+  constexpr int MT = PACKED ? 8 / P : 8 * NT;   // most rows of a block
+  constexpr int TURNS = (MT + 1) / 2;           // rows of a half warp
+  const W4 w = p.w;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % sp.cluster, kb = blockIdx.x / sp.cluster;
+  const int m0 = blockIdx.y * sp.tile_m, M = min(sp.tile_m, p.M - m0);
+  const int cv = PACKED ? M * P : (NT == 1 ? M : 8);
+  const int tiles = (w.n_out + TILE_N - 1) / TILE_N, share = (tiles + sp.cluster - 1) / sp.cluster;
+  const int first = min(rank * share, tiles), end = min(first + share, tiles);
+  const int groups = w.groups();
+  const long long pitch = w.pitch();
+  const uint32_t ring = smem_of(smem) + warp * (STAGES * STAGE_BYTES);
+  const int set_bytes = Q * cv * 64;
+  const uint32_t as = smem_of(smem) + RING_BYTES + warp * (SETS * set_bytes);  // [set][part, tile][column][32 outputs, in the order the lanes read them]
+  // a lane makes the parts of two neighbouring outputs of every other row
+  const int pair = lane & 15, odd = lane >> 4, in8 = pair & 7;
+  const uint32_t place = as + ((pair >> 3) * 16 + (in8 & 3) * 4 + (in8 >> 2) * 2) * 2;
+  const int size = p.type == BF_TYPE_F32 ? 4 : 2;
+  const bool wide = w.n_out % 2 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & (2 * size - 1)) == 0;
+  const uint8_t* codes = w.codes + (long long)kb * (CHUNK / 2) + (lane & 3) * 16;
+  const int bytes = (int)min((long long)CHUNK, pitch - (long long)kb * (CHUNK / 2));
+
+  float acc[SETS][4][2][NT][4];
+#pragma unroll
+  for (int s = 0; s < SETS; ++s)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[s][r][e][j][i] = 0.f;
+
+  auto rows_at = [&](int tile, float (&v)[SETS][TURNS][2]) {
+    const int n = tile * TILE_N + 2 * pair;
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      const int m = 2 * i + odd;
+#pragma unroll
+      for (int s = 0; s < SETS; ++s) v[s][i][0] = v[s][i][1] = 0.f;
+      if (m < M && tile < end && n < w.n_out) {
+        const long long at = (long long)(m0 + m) * w.n_out + n;
+        const bool two = n + 1 < w.n_out;
+        if (P == 3) {
+#pragma unroll
+          for (int s = 0; s < SETS; ++s) {
+            const float* from = (s == 0 ? static_cast<const float*>(p.a) : p.b) + at;
+            if (wide) {
+              const float2 f = *reinterpret_cast<const float2*>(from);
+              v[s][i][0] = f.x;
+              v[s][i][1] = f.y;
+            } else {
+              v[s][i][0] = from[0];
+              if (two) v[s][i][1] = from[1];
+            }
+          }
+        } else {
+          uint32_t q;
+          const uint16_t* from = static_cast<const uint16_t*>(p.a) + at;
+          if (wide) q = *reinterpret_cast<const uint32_t*>(from);
+          else q = from[0] | (two ? (uint32_t)from[1] << 16 : 0u);
+          const float2 f = p.type == BF_TYPE_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q)) : __half22float2(*reinterpret_cast<const __half2*>(&q));
+          v[0][i][0] = f.x;
+          v[0][i][1] = f.y;
+        }
+      }
+    }
+  };
+
+  int next = first + warp;
+  auto load_next = [&](uint32_t to) {
+    if (next < end) {
+      const int n0 = next * TILE_N, rows = min(TILE_N, w.n_out - n0);
+      load_codes(to, codes + (long long)(n0 + min(lane >> 2, rows - 1)) * pitch, 8 * pitch, rows, bytes, lane);
+      load_scales(to, w, groups, n0, kb, lane);
+    }
+    copies_begin();
+    next += WARPS;
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) load_next(ring + s * STAGE_BYTES);
+  float av[SETS][TURNS][2];
+  rows_at(first + warp, av);
+  int slot = 0;
+  for (int tile = first + warp; tile < end; tile += WARPS) {
+    float now[SETS][TURNS][2];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (DUAL) {  // gradients of lower and upper bounds to those of centre and radius
+          now[0][i][j] = av[0][i][j] + av[SETS - 1][i][j];
+          now[SETS - 1][i][j] = av[SETS - 1][i][j] - av[0][i][j];
+        } else {
+          now[0][i][j] = av[0][i][j];
+        }
+      }
+    rows_at(tile + WARPS, av);
+    copies_wait<STAGES - 2>();
+    __syncwarp();
+    load_next(ring + (slot == 0 ? STAGES - 1 : slot - 1) * STAGE_BYTES);
+    const uint32_t st = ring + slot * STAGE_BYTES;
+    slot = slot == STAGES - 1 ? 0 : slot + 1;
+#pragma unroll
+    for (int group = 0; group < 4 / STEPS; ++group) {
+      {
+        const uint32_t at = st + TILE_N * ROW_BYTES + (group * TILE_N + 2 * pair) * 4;
+        const float f0 = __uint_as_float(lds32(at)), f1 = __uint_as_float(lds32(at + 4));
+        if (group > 0) __syncwarp();
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+          const int m = 2 * i + odd;
+          if (m < M) {
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) {
+              uint32_t q[P];
+              two_numbers_checked<P>(now[s][i][0] * (s == 0 ? f0 : fabsf(f0)), now[s][i][1] * (s == 0 ? f1 : fabsf(f1)), q);
+#pragma unroll
+              for (int part = 0; part < P; ++part) {
+                const int j = PACKED ? m * P + part : part * NT * 8 + m;
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(place + s * set_bytes + ((j >> 3) * cv + (j & 7)) * 64), "r"(q[part]) : "memory");
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t b[SETS][Q][2];
+#pragma unroll
+        for (int s = 0; s < SETS; ++s)
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];"
+                         : "=r"(b[s][q][0]), "=r"(b[s][q][1])
+                         : "r"(as + s * set_bytes + ((q * cv + min(g, cv - 1)) * 32 + h * 16 + 4 * t) * 2)
+                         : "memory");
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          const int step = group * STEPS + i;
+          const uint32_t row = st + (h * 16 + 2 * t) * ROW_BYTES + (step * 4 + (g & 3)) * 4;
+          const uint32_t w0 = lds32(row), w1 = lds32(row + ROW_BYTES), w8 = lds32(row + 8 * ROW_BYTES), w9 = lds32(row + 9 * ROW_BYTES);
+          const uint32_t sel = g >= 4 ? 0x7632u : 0x5410u;
+          const uint32_t lo = __byte_perm(w0, w1, sel), hi = __byte_perm(w8, w9, sel);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t a[4] = {weights_of(lo >> (8 * e)), weights_of(lo >> (8 * e + 4)), weights_of(hi >> (8 * e)), weights_of(hi >> (8 * e + 4))};
+#pragma unroll
+            for (int q = 0; q < Q; ++q) mma(acc[0][step][e][q % NT], a[0], a[1], a[2], a[3], b[0][q][0], b[0][q][1]);
+            if (DUAL) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) a[k] &= 0x7fff7fffu;
+#pragma unroll
+              for (int q = 0; q < Q; ++q) mma(acc[SETS - 1][step][e][q % NT], a[0], a[1], a[2], a[3], b[SETS - 1][q][0], b[SETS - 1][q][1]);
+            }
+          }
+        }
+      }
+    }
+  }
+  // Sums over the warps, eight columns of rows at a time, then over the blocks of the cluster, each in order.
+  float* red = reinterpret_cast<float*>(smem);  // [warp][8][128 and a pad]
+  constexpr int LINE = CHUNK + 4;
+  float* own = red + WARPS * 8 * LINE;          // [product][row][128]
+  copies_wait<0>();
+#pragma unroll
+  for (int s = 0; s < SETS; ++s)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            red[(warp * 8 + 2 * t + (i & 1)) * LINE + r * 32 + 8 * (g & 3) + 4 * (g >> 2) + 2 * e + (i >> 1)] = acc[s][r][e][j][i];
+      __syncthreads();
+      const int here = PACKED ? M : min(8, M - j * 8);  // rows of the tile
+      for (int i = threadIdx.x; i < here * CHUNK; i += THREADS) {
+        const int m = i / CHUNK, k = i % CHUNK;
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < (PACKED ? P : 1); ++q)
+#pragma unroll
+          for (int x = 0; x < WARPS; ++x) v += red[(x * 8 + (PACKED ? m * P + q : m)) * LINE + k];
+        own[(s * M + j * 8 + m) * CHUNK + k] = v;
+      }
+    }
+  if (sp.cluster > 1) cluster_barrier();
+  else __syncthreads();
+  const int mine = CHUNK / sp.cluster;
+  for (int i = threadIdx.x; i < mine * M; i += THREADS) {
+    const int m = i / mine, k = rank * mine + i - m * mine;
+    if (kb * CHUNK + k >= w.n_in) continue;
+    float sum[2];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) sum[s] = cluster_sum(own + (s * M + m) * CHUNK + k, sp.cluster);
+    const long long at = (long long)(m0 + m) * w.n_in + kb * CHUNK + k;
+    if (DUAL) {
+      static_cast<float*>(p.z)[at] = 0.5f * (sum[0] - sum[1]);
+      p.z2[at] = 0.5f * (sum[0] + sum[1]);
+    } else {
+      store_any(p.z, p.type, at, sum[0]);
+    }
+  }
+  if (sp.cluster > 1) cluster_barrier();
+}
+
+template <int P, bool PACKED, int NT, bool DUAL>
+int backward(const W4RowsArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
+  static SmemOptIn table[3];
+  const int kblocks = ceil_div(p.w.n_in, CHUNK), tiles = ceil_div(p.w.n_out, TILE_N);
+  const long long units = (long long)kblocks * tiles_m;
+  const int split = (int)std::max<long long>(1, std::min<long long>(ceil_div(tiles, WARPS), (2LL * SMS) / units));
+  sp.cluster = std::min(8, power_below(split));
+  const int cv = PACKED ? sp.tile_m * P : (NT == 1 ? sp.tile_m : 8);
+  const int rows_bytes = WARPS * (DUAL ? 2 : 1) * (PACKED ? 1 : P * NT) * cv * 64;
+  const int smem = RING_BYTES + rows_bytes;  // (the sums at the end need less)
+  const long long blocks = (long long)kblocks * sp.cluster;
+  if (p.w.group_log2 == 5) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 1>, "w4_rows_kernel", table[0], p, sp, blocks, tiles_m, smem, stream);
+  if (p.w.group_log2 == 6) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 2>, "w4_rows_kernel", table[1], p, sp, blocks, tiles_m, smem, stream);
+  return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 4>, "w4_rows_kernel", table[2], p, sp, blocks, tiles_m, smem, stream);
+}
+
+}  // namespace
+
+int launch_w4_rows(const W4RowsArgs& all, cudaStream_t stream) {
+  Split sp = {};
+  const int parts = all.type == BF_TYPE_F32 ? 3 : 2;  // a 16-bit row times a 32-bit scale: two parts hold it to 2^-18
+  const bool dual = all.b != nullptr;
+  sp.packed = all.M * parts <= 8;
+  const int nt = dual || sp.packed || all.M <= 8 ? 1 : 2;
+  sp.tile_m = std::min(all.M, 8 * nt);
+  const long long tiles = ceil_div(all.M, sp.tile_m);
+  for (long long first = 0; first < tiles; first += MOST_TILES) {
+    const int here = (int)std::min<long long>(MOST_TILES, tiles - first);
+    W4RowsArgs p = all;
+    const long long skip = first * sp.tile_m, size = all.type == BF_TYPE_F32 ? 4 : 2;
+    p.M = (int)std::min<long long>(all.M - skip, (long long)here * sp.tile_m);
+    p.a = static_cast<const char*>(all.a) + skip * all.w.n_out * size;
+    p.b = dual ? all.b + skip * all.w.n_out : nullptr;
+    p.z = static_cast<char*>(all.z) + skip * all.w.n_in * size;
+    p.z2 = dual ? all.z2 + skip * all.w.n_in : nullptr;
+    int rc;
+    if (dual) rc = sp.packed ? backward<3, true, 1, true>(p, sp, here, stream) : backward<3, false, 1, true>(p, sp, here, stream);
+    else if (sp.packed) rc = parts == 3 ? backward<3, true, 1, false>(p, sp, here, stream) : backward<2, true, 1, false>(p, sp, here, stream);
+    else if (parts == 2) rc = nt == 1 ? backward<2, false, 1, false>(p, sp, here, stream) : backward<2, false, 2, false>(p, sp, here, stream);
+    else rc = nt == 1 ? backward<3, false, 1, false>(p, sp, here, stream) : backward<3, false, 2, false>(p, sp, here, stream);
+    if (rc != BF_OK) return rc;
+  }
+  return BF_OK;
+}
+
+}  // namespace bf
