@@ -178,6 +178,7 @@ def _exact_arity(fn, n_args: int, name: str):
 
     call.__name__ = name
     call.restype, call.argtypes = fn.restype, fn.argtypes
+    call.unchecked = fn  # for callers within the package that pass a fixed list and count microseconds
     return call
 
 

@@ -49,67 +49,116 @@ struct AdamCommon {
   int last;
 };
 
-template <typename T> struct Four;
-template <> struct Four<float> { using type = float4; };
-template <> struct Four<__nv_bfloat16> { using type = uint2; };
-template <> struct Four<__half> { using type = uint2; };
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ void put(float& d, float v) { d = v; }
-__device__ __forceinline__ void put(__nv_bfloat16& d, float v) { d = __float2bfloat16(v); }
-__device__ __forceinline__ void put(__half& d, float v) { d = __float2half(v); }
+// A lane's eight elements of a block, four at 4 * lane and four at 128 + 4 * lane, as they lie in memory.
+template <typename T> struct Eight { using Four = uint2; Four q[2]; };
+template <> struct Eight<float> { using Four = uint4; Four q[2]; };
 
-// A lane's eight elements of a block: four at 4 * lane, four at 128 + 4 * lane.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int lane, int left, bool wide, float (&x)[8]) {
+__device__ __forceinline__ Eight<T> load8(const T* p, int lane, int left, bool wide) {
+  Eight<T> r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int at = h * 128 + lane * 4;
     if (wide && at + 4 <= left) {
-      typename Four<T>::type q = *reinterpret_cast<const typename Four<T>::type*>(p + at);
-      const T* t = reinterpret_cast<const T*>(&q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * h + i] = to_f(t[i]);
+      r.q[h] = *reinterpret_cast<const typename Eight<T>::Four*>(p + at);
     } else {
+      T t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * h + i] = at + i < left ? to_f(p[at + i]) : 0.f;
+      for (int i = 0; i < 4; ++i) t[i] = at + i < left ? p[at + i] : T(0.f);
+      memcpy(&r.q[h], t, sizeof t);
     }
   }
+  return r;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int lane, int left, bool wide, const float (&x)[8]) {
+__device__ __forceinline__ void store8(T* p, int lane, int left, bool wide, const Eight<T>& r) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int at = h * 128 + lane * 4;
-    T t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) put(t[i], x[4 * h + i]);
     if (wide && at + 4 <= left) {
-      typename Four<T>::type q;
-      memcpy(&q, t, sizeof q);
-      *reinterpret_cast<typename Four<T>::type*>(p + at) = q;
+      *reinterpret_cast<typename Eight<T>::Four*>(p + at) = r.q[h];
     } else {
+      T t[4];
+      memcpy(t, &r.q[h], sizeof t);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (at + i < left) p[at + i] = t[i];
     }
   }
 }
+__device__ __forceinline__ void numbers(const Eight<float>& r, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    x[4 * h] = __uint_as_float(r.q[h].x);
+    x[4 * h + 1] = __uint_as_float(r.q[h].y);
+    x[4 * h + 2] = __uint_as_float(r.q[h].z);
+    x[4 * h + 3] = __uint_as_float(r.q[h].w);
+  }
+}
+__device__ __forceinline__ void numbers(const Eight<__nv_bfloat16>& r, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    x[4 * h] = __uint_as_float(r.q[h].x * 65536u);
+    x[4 * h + 1] = __uint_as_float(r.q[h].x & 0xffff0000u);
+    x[4 * h + 2] = __uint_as_float(r.q[h].y * 65536u);
+    x[4 * h + 3] = __uint_as_float(r.q[h].y & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void numbers(const Eight<__half>& r, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.q[h].x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.q[h].y));
+    x[4 * h] = a.x;
+    x[4 * h + 1] = a.y;
+    x[4 * h + 2] = b.x;
+    x[4 * h + 3] = b.y;
+  }
+}
+__device__ __forceinline__ uint32_t two(__nv_bfloat16*, float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t two(__half*, float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> rounded(const float (&x)[8]) {
+  Eight<T> r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) r.q[h] = make_uint2(two(static_cast<T*>(nullptr), x[4 * h], x[4 * h + 1]), two(static_cast<T*>(nullptr), x[4 * h + 2], x[4 * h + 3]));
+  return r;
+}
+template <>
+__device__ __forceinline__ Eight<float> rounded<float>(const float (&x)[8]) {
+  Eight<float> r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    r.q[h] = make_uint4(__float_as_uint(x[4 * h]), __float_as_uint(x[4 * h + 1]), __float_as_uint(x[4 * h + 2]), __float_as_uint(x[4 * h + 3]));
+  return r;
+}
 
 // ---- 8-bit moments -----------------------------------------------------------------
+// Integer work is what the 8-bit step is short of (64 lanes a clock, half of what FP32 has): codes are kept where a byte permutation finds them, shifts to the left
+// are multiplications (which run beside it), and signs and zeros are dealt with for four codes at a time.
 constexpr int M_FIELDS = 15, V_FIELDS = 31;  // powers of two below the block's exponent
 
-__device__ __forceinline__ uint32_t rounding_noise(uint32_t place, uint32_t step) {
-  uint32_t x = place ^ (step * 0x9E3779B1u);
+__device__ __forceinline__ uint32_t rounding_noise(uint32_t place, uint32_t key) {
+  uint32_t x = place ^ key;
   x = (x ^ (x >> 16)) * 0x9BC84D59u;
   x = (x ^ (x >> 15)) * 0x7641A5C5u;
   return x ^ (x >> 16);
 }
-template <int FIELDS>
-__device__ __forceinline__ float decode(uint32_t code, int e) {
-  if (e == 255) return __int_as_float(0x7fffffff);
-  return code == 0 ? 0.f : __uint_as_float((code + ((uint32_t)(e - FIELDS) << 3)) << 20);
+// The four numbers of `word`; a code is added to the bit pattern of the power of two below its range.
+template <int FIELDS, bool SIGNED>
+__device__ __forceinline__ void decode4(uint32_t word, int exponent, float* x) {
+  const uint32_t base = (uint32_t)(exponent - FIELDS) << 23, codes = SIGNED ? word & 0x7f7f7f7fu : word;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t c = __byte_perm(codes, 0, 0x4044 | (i << 8));  // the code in bits 16-23
+    const uint32_t bits = (c * 16 + base) * min(c, 1u);
+    x[i] = __uint_as_float(SIGNED ? bits | ((word * (1u << (24 - 8 * i))) & 0x80000000u) : bits);
+  }
 }
 // `top`: bit pattern of the block's largest magnitude.
 template <int FIELDS>
@@ -117,111 +166,189 @@ __device__ __forceinline__ int shared_exponent(uint32_t top) {
   if (top >= 0x7f800000u) return 255;
   return min(254, max(FIELDS + 1, (int)((top + 0xfffffu) >> 23)));
 }
+// Four codes: magnitude and 20 bits of noise, counted from the power of two below the range; the code is what is above bit 20.  Nothing is above the largest
+// code, as the exponent is chosen.
+template <int FIELDS, bool SIGNED>
+__device__ __forceinline__ uint32_t encode4(const float* x, const uint32_t (&noise20)[4], int exponent) {
+  const uint32_t base = (uint32_t)(exponent - FIELDS) << 23;
+  uint32_t d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bits = __float_as_uint(x[i]);
+    const int v = (int)((SIGNED ? bits & 0x7fffffffu : bits) + noise20[i] - base);
+    d[i] = (uint32_t)max(v, SIGNED ? 0 : (int)(min(bits, 1u) * (1u << 20))) * 16;  // a second moment that is not zero keeps a code that is not
+  }
+  uint32_t word = __byte_perm(__byte_perm(d[0], d[1], 0x0073), __byte_perm(d[2], d[3], 0x0073), 0x5410);
+  if (SIGNED) {
+    const uint32_t signs = __byte_perm(__byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0073), __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0073), 0x5410);
+    word |= (word + 0x7f7f7f7fu) & signs & 0x80808080u;  // zero has no sign
+  }
+  return word;
+}
+// Where the largest exponent is cut (254), magnitudes above the largest code are cut to it.
 template <int FIELDS>
-__device__ __forceinline__ uint32_t encode(float magnitude, uint32_t noise20, int e) {
-  const int rel = (int)((__float_as_uint(magnitude) + noise20) >> 20) - ((e - FIELDS) << 3);
-  return (uint32_t)min(8 * FIELDS + 7, max(0, rel));
+__device__ __forceinline__ void cut(float (&x)[8]) {
+  const float most = __uint_as_float(((uint32_t)(254 - FIELDS) << 23) + ((8u * FIELDS + 7u) << 20));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = copysignf(fminf(fabsf(x[i]), most), x[i]);
 }
 
+// Root and quotient of the step itself need no more than the approximations' 2^-22: the step is far below the parameter.  Numbers below the normal range
+// count as zero in them, which an eps above 1e-18 covers.
+__device__ __forceinline__ float quotient(float m, float v, float root, float eps) {
+  float s, q;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+  asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(s, root, eps)));
+  return q;
+}
+
+// A warp's work of a turn: where it lies, and for 8-bit moments all that it reads, fetched a turn ahead.
+template <typename P, typename G>
+struct Turn {
+  long long at, slot;
+  int entry, left;  // left <= 0: nothing to do
+  Eight<P> p;
+  Eight<G> g;
+  uint32_t m[2], v[2];
+  int me, ve;
+};
+
 template <typename P, typename G, bool EIGHT, int CAP>
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamTable<CAP> tab, const AdamCommon c) {
+__global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_constant__ AdamTable<CAP> tab, const AdamCommon c) {
   __shared__ float sh_rate, sh_root, sh_scale;
-  __shared__ uint32_t sh_step;
+  __shared__ uint32_t sh_key;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    const double q1 = c.state[0] * c.beta1, q2 = c.state[1] * c.beta2;
-    sh_rate = (float)(1.0 / (1.0 - q1));
-    sh_root = (float)(1.0 / sqrt(1.0 - q2));
-    sh_step = (uint32_t)(c.state[2] + 1.0);
-    sh_scale = c.grad_scale ? *c.grad_scale : 1.f;
-  }
-  __syncthreads();
-  const float rate = sh_rate, root = sh_root, scale = sh_scale;
-  const uint32_t step = sh_step;
-  int t = 0;
-  for (unsigned chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
-    if (t + 1 < tab.count && chunk >= tab.e[t + 1].chunk0) {  // the last tensor that begins at or before this chunk
-      int lo = t + 1, hi = tab.count;
+  int near = 0;  // the tensor of the last chunk that was looked up
+  auto locate = [&](unsigned chunk, Turn<P, G>& w) {
+    if (near + 1 < tab.count && chunk >= tab.e[near + 1].chunk0) {  // the last tensor that begins at or before this chunk
+      int lo = near + 1, hi = tab.count;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (chunk >= tab.e[mid].chunk0) lo = mid;
         else hi = mid;
       }
-      t = lo;
+      near = lo;
     }
-    const AdamEntry& e = tab.e[t];
-    const long long at = (long long)(chunk - e.chunk0) * CHUNK + warp * BLOCK;
-    if (at >= e.n) continue;
-    const int left = (int)min((long long)BLOCK, e.n - at);
-    P* p = static_cast<P*>(e.p) + at;
-    const G* g = static_cast<const G*>(e.g) + at;
-    const bool wide_p = (reinterpret_cast<uintptr_t>(e.p) & (4 * sizeof(P) - 1)) == 0, wide_g = (reinterpret_cast<uintptr_t>(e.g) & (4 * sizeof(G) - 1)) == 0;
-    const long long slot = e.first + at;
-    float pv[8], gv[8], m[8], v[8];
-    load8(p, lane, left, wide_p, pv);
-    load8(g, lane, left, wide_g, gv);
+    const AdamEntry& e = tab.e[near];
+    w.entry = near;
+    w.at = (long long)(chunk - e.chunk0) * CHUNK + warp * BLOCK;
+    w.slot = e.first + w.at;
+    w.left = (int)min((long long)BLOCK, e.n - w.at);
+  };
+  auto fetch = [&](Turn<P, G>& w) {
+    const AdamEntry& e = tab.e[w.entry];
+    w.p = load8(static_cast<const P*>(e.p) + w.at, lane, w.left, (reinterpret_cast<uintptr_t>(e.p) & (4 * sizeof(P) - 1)) == 0);
+    w.g = load8(static_cast<const G*>(e.g) + w.at, lane, w.left, (reinterpret_cast<uintptr_t>(e.g) & (4 * sizeof(G) - 1)) == 0);
     if (EIGHT) {
-      const int me = c.me[slot / BLOCK], ve = c.ve[slot / BLOCK];
-      const uint8_t *m8 = static_cast<const uint8_t*>(c.m) + slot, *v8 = static_cast<const uint8_t*>(c.v) + slot;
+      w.me = c.me[w.slot / BLOCK];
+      w.ve = c.ve[w.slot / BLOCK];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t mw = *reinterpret_cast<const uint32_t*>(m8 + h * 128 + lane * 4), vw = *reinterpret_cast<const uint32_t*>(v8 + h * 128 + lane * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t mc = (mw >> (8 * i)) & 255u, vc = (vw >> (8 * i)) & 255u;
-          const float size = decode<M_FIELDS>(mc & 127u, me);
-          m[4 * h + i] = (mc & 128u) ? -size : size;
-          v[4 * h + i] = decode<V_FIELDS>(vc, ve);
-        }
+        w.m[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.m) + w.slot + h * 128 + lane * 4);
+        w.v[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.v) + w.slot + h * 128 + lane * 4);
       }
-    } else {
-      load8(static_cast<const float*>(c.m) + slot, lane, BLOCK, true, m);
-      load8(static_cast<const float*>(c.v) + slot, lane, BLOCK, true, v);
     }
-    const float rate_lr = -e.lr * rate, decay = e.decay;
+  };
+  unsigned chunk = blockIdx.x;
+  Turn<P, G> now;
+  now.left = 0;
+  if (chunk < tab.chunks) {
+    locate(chunk, now);
+    if (EIGHT && now.left > 0) fetch(now);
+  }
+  if (threadIdx.x == 0) {
+    const double q1 = c.state[0] * c.beta1, q2 = c.state[1] * c.beta2;
+    sh_rate = (float)(1.0 / (1.0 - q1));
+    sh_root = (float)(1.0 / sqrt(1.0 - q2));
+    sh_key = (uint32_t)(c.state[2] + 1.0) * 0x9E3779B1u;
+    sh_scale = c.grad_scale ? *c.grad_scale : 1.f;
+  }
+  __syncthreads();
+  const float rate = sh_rate, root = sh_root, scale = sh_scale;
+  const uint32_t key = sh_key;
+  while (chunk < tab.chunks) {
+    Turn<P, G> then;
+    then.left = 0;
+    const unsigned next = chunk + gridDim.x;
+    if (next < tab.chunks) {
+      locate(next, then);
+      if (EIGHT && then.left > 0) fetch(then);
+    }
+    if (now.left > 0) {
+      const AdamEntry& e = tab.e[now.entry];
+      float p[8], g[8], m[8], v[8];
+      if (EIGHT) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gi = __fmul_rn(gv[i], scale);
-      m[i] = __fadd_rn(__fmul_rn(c.b1, m[i]), __fmul_rn(c.c1, gi));
-      v[i] = __fadd_rn(__fmul_rn(c.b2, v[i]), __fmul_rn(__fmul_rn(c.c2, gi), gi));
-      pv[i] = fmaf(rate_lr, m[i] / fmaf(sqrtf(v[i]), root, c.eps), pv[i] * decay);
-    }
-    store8(p, lane, left, wide_p, pv);
-    if (EIGHT) {
-      uint32_t mt = 0, vt = 0;
+        for (int h = 0; h < 2; ++h) {
+          decode4<M_FIELDS, true>(now.m[h], now.me, m + 4 * h);
+          decode4<V_FIELDS, false>(now.v[h], now.ve, v + 4 * h);
+        }
+        if (max(now.me, now.ve) == 255) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (now.me == 255) m[i] = __int_as_float(0x7fffffff);
+            if (now.ve == 255) v[i] = __int_as_float(0x7fffffff);
+          }
+        }
+      } else {
+        fetch(now);
+        numbers(load8(static_cast<const float*>(c.m) + now.slot, lane, BLOCK, true), m);
+        numbers(load8(static_cast<const float*>(c.v) + now.slot, lane, BLOCK, true), v);
+      }
+      numbers(now.p, p);
+      numbers(now.g, g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        mt = max(mt, __float_as_uint(m[i]) & 0x7fffffffu);
-        vt = max(vt, __float_as_uint(v[i]) & 0x7fffffffu);
+        const float gi = __fmul_rn(g[i], scale);
+        m[i] = __fadd_rn(__fmul_rn(c.b1, m[i]), __fmul_rn(c.c1, gi));
+        v[i] = __fadd_rn(__fmul_rn(c.b2, v[i]), __fmul_rn(__fmul_rn(c.c2, gi), gi));
       }
-      mt = __reduce_max_sync(0xffffffffu, mt);
-      vt = __reduce_max_sync(0xffffffffu, vt);
-      const int me = shared_exponent<M_FIELDS>(mt), ve = shared_exponent<V_FIELDS>(vt);
-      uint8_t *m8 = static_cast<uint8_t*>(c.m) + slot, *v8 = static_cast<uint8_t*>(c.v) + slot;
+      const float step = -e.lr * rate, decay = e.decay;
+      if (c.eps > 1e-18f) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t mw = 0, vw = 0;
+        for (int i = 0; i < 8; ++i) p[i] = fmaf(step, quotient(m[i], v[i], root, c.eps), p[i] * decay);
+      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float mi = m[4 * h + i], vi = v[4 * h + i];
-          const uint32_t noise = rounding_noise((uint32_t)(slot + h * 128 + lane * 4 + i), step);
-          const uint32_t mc = encode<M_FIELDS>(fabsf(mi), noise & 0xfffffu, me);
-          uint32_t vc = encode<V_FIELDS>(vi, noise >> 12, ve);
-          if (vi > 0.f && vc == 0) vc = 1;
-          mw |= (mc | (mc != 0 && mi < 0.f ? 128u : 0u)) << (8 * i);
-          vw |= vc << (8 * i);
+        for (int i = 0; i < 8; ++i) p[i] = fmaf(step, m[i] / fmaf(sqrtf(v[i]), root, c.eps), p[i] * decay);
+      }
+      store8(static_cast<P*>(e.p) + now.at, lane, now.left, (reinterpret_cast<uintptr_t>(e.p) & (4 * sizeof(P) - 1)) == 0, rounded<P>(p));
+      if (EIGHT) {
+        uint32_t mt = 0, vt = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          mt = max(mt, __float_as_uint(m[i]) & 0x7fffffffu);
+          vt = max(vt, __float_as_uint(v[i]));  // never negative
         }
-        *reinterpret_cast<uint32_t*>(m8 + h * 128 + lane * 4) = mw;
-        *reinterpret_cast<uint32_t*>(v8 + h * 128 + lane * 4) = vw;
+        mt = __reduce_max_sync(0xffffffffu, mt);
+        vt = __reduce_max_sync(0xffffffffu, vt & 0x7fffffffu);
+        const int me = shared_exponent<M_FIELDS>(mt), ve = shared_exponent<V_FIELDS>(vt);
+        if (max(me, ve) >= 254) {
+          cut<M_FIELDS>(m);
+          cut<V_FIELDS>(v);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t low[4], high[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t noise = rounding_noise((uint32_t)(now.slot + h * 128 + lane * 4) ^ (uint32_t)i, key);  // (a multiple of four, so this is + i)
+            low[i] = noise & 0xfffffu;
+            high[i] = noise >> 12;
+          }
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(c.m) + now.slot + h * 128 + lane * 4) = encode4<M_FIELDS, true>(m + 4 * h, low, me);
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(c.v) + now.slot + h * 128 + lane * 4) = encode4<V_FIELDS, false>(v + 4 * h, high, ve);
+        }
+        if (lane == 0) {
+          c.me[now.slot / BLOCK] = (uint8_t)me;
+          c.ve[now.slot / BLOCK] = (uint8_t)ve;
+        }
+      } else {
+        store8(static_cast<float*>(c.m) + now.slot, lane, BLOCK, true, rounded<float>(m));
+        store8(static_cast<float*>(c.v) + now.slot, lane, BLOCK, true, rounded<float>(v));
       }
-      if (lane == 0) {
-        c.me[slot / BLOCK] = (uint8_t)me;
-        c.ve[slot / BLOCK] = (uint8_t)ve;
-      }
-    } else {
-      store8(static_cast<float*>(c.m) + slot, lane, BLOCK, true, m);
-      store8(static_cast<float*>(c.v) + slot, lane, BLOCK, true, v);
     }
+    chunk = next;
+    now = then;
   }
   // The step's last launch counts it: every block has read the count when it arrives here, the last to arrive moves it on.
   if (c.last && threadIdx.x == 0) {
@@ -240,21 +367,20 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* m8, const uint8_t* v8, const uint8_t* me, const uint8_t* ve, __nv_bfloat16* m,
                                                             __nv_bfloat16* v, long long n) {
   for (long long i = (blockIdx.x * 256LL + threadIdx.x) * 4; i < n; i += gridDim.x * 1024LL) {
-    const uint32_t mw = *reinterpret_cast<const uint32_t*>(m8 + i), vw = *reinterpret_cast<const uint32_t*>(v8 + i);
-    const int em = me[i / BLOCK], ev = ve[i / BLOCK];
     float a[4], b[4];
+    const int em = me[i / BLOCK], ev = ve[i / BLOCK];
+    decode4<M_FIELDS, true>(*reinterpret_cast<const uint32_t*>(m8 + i), em, a);
+    decode4<V_FIELDS, false>(*reinterpret_cast<const uint32_t*>(v8 + i), ev, b);
+    if (max(em, ev) == 255) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t mc = (mw >> (8 * j)) & 255u;
-      const float size = decode<M_FIELDS>(mc & 127u, em);
-      a[j] = (mc & 128u) ? -size : size;
-      b[j] = decode<V_FIELDS>((vw >> (8 * j)) & 255u, ev);
+      for (int j = 0; j < 4; ++j) {
+        if (em == 255) a[j] = __int_as_float(0x7fffffff);
+        if (ev == 255) b[j] = __int_as_float(0x7fffffff);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m[i + j] = __float2bfloat16(a[j]);
-      v[i + j] = __float2bfloat16(b[j]);
-    }
+    __nv_bfloat162 o[4] = {__floats2bfloat162_rn(a[0], a[1]), __floats2bfloat162_rn(a[2], a[3]), __floats2bfloat162_rn(b[0], b[1]), __floats2bfloat162_rn(b[2], b[3])};
+    *reinterpret_cast<uint2*>(m + i) = *reinterpret_cast<const uint2*>(o);
+    *reinterpret_cast<uint2*>(v + i) = *reinterpret_cast<const uint2*>(o + 2);
   }
 }
 
@@ -269,7 +395,7 @@ int launch(const bf_adamw_tensor* t, int count, const AdamCommon& c, cudaStream_
   BF_REQUIRE(chunks < (1ULL << 31), BF_E_UNSUPPORTED, "bf_adamw_step: more than 2^42 elements in one launch");
   tab.count = count;
   tab.chunks = (unsigned)chunks;
-  const int cap = 148 * 8, grid = chunks == 0 ? 1 : chunks < (unsigned)cap ? (int)chunks : cap;
+  const int cap = 148 * (EIGHT ? 3 : 4), grid = chunks == 0 ? 1 : chunks < (unsigned)cap ? (int)chunks : cap;
   adamw_kernel<P, G, EIGHT, CAP><<<grid, 256, 0, stream>>>(tab, c);
   BF_CHECK_LAUNCH("adamw_kernel");
   return BF_OK;

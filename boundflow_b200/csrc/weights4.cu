@@ -7,44 +7,138 @@ namespace bf {
 namespace {
 
 // ---- quantisation ----------------------------------------------------------------
-// A warp per (row, group): largest magnitude, scale = that times 1/7 (as a 32-bit number), codes = round(w / scale) + 8.  The largest is taken over bit patterns, whose
-// order is that of the magnitudes with infinities and NaN above: a group that holds one has it as its scale and is NaN throughout.
+__device__ __forceinline__ void load_eight(const void* p, int type, long long at, int left, bool wide, float (&v)[8]) {
+  if (!wide || left < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? load_any(p, type, at + j) : 0.f;
+  } else if (type == BF_TYPE_F32) {
+    const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at), y = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+    const uint32_t q[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = type == BF_TYPE_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[j])) : __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+// Bit pattern of the largest magnitude, that of a NaN where an infinity or a NaN is among them.
+__device__ __forceinline__ uint32_t largest(const float (&v)[8]) {
+  float top = 0.f, finite = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    top = fmaxf(top, fabsf(v[j]));
+    finite = fmaf(v[j], 0.f, finite);
+  }
+  return finite == 0.f ? __float_as_uint(top) : 0x7fc00000u;
+}
+// Eight codes.  The quotient is the rounded one of a division by definition; a product with the reciprocal is within 2^-20 of it, so that both round to the same
+// whole number unless they lie that near to half of one: those are divided.  Adding 1.5 * 2^23 rounds to a whole number and leaves it, + 8, in the last bits, which
+// are collected with products: what the sum of the constants' own bits comes to is taken off at the end.
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[8], float scale, float inverse) {
+  constexpr float MAGIC = 12582912.f + 8.f;
+  if (!(scale > 0.f && scale < INFINITY)) return 0x88888888u;  // zeros, or a group that its scale makes NaN
+  float off = inverse < INFINITY ? 0.f : 1.f;
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) {
+    const float t = fmaf(v[j], inverse, MAGIC);
+    off = fmaxf(off, fabsf(fmaf(v[j], inverse, MAGIC - t)));
+    word = word * 16u + __float_as_uint(t);
+  }
+  if (off > 0.49999f) {
+    word = 0;
+#pragma unroll
+    for (int j = 7; j >= 0; --j) word = word * 16u + (uint32_t)(__float2int_rn(fminf(fmaxf(rintf(__fdiv_rn(v[j], scale)), -7.f), 7.f)) + 8);
+    return word;
+  }
+  return word - 0x4B400000u * 0x11111111u;
+}
+
+// Largest magnitude of a group, scale = that times 1/7 (as a 32-bit number), codes = round(w / scale) + 8.  The largest is taken over bit patterns, whose order
+// is that of the magnitudes with infinities and NaN above: a group that holds one has it as its scale and is NaN throughout.
+// A thread takes eight neighbours; as many lanes as a group of up to 256 needs share its largest (groups do not straddle warps).
 __global__ void __launch_bounds__(256) w4_quantise_kernel(const void* W, int type, uint8_t* codes, float* scales, W4 w) {
-  const int G = 1 << w.group_log2, lane = threadIdx.x & 31;
-  const int groups = w.groups();
+  const unsigned per_row = (unsigned)((w.groups() << w.group_log2) >> 3);
+  const int lanes = 1 << (w.group_log2 - 3);
+  const long long units = (long long)w.n_out * per_row, stride = (long long)gridDim.x * 256;
+  const bool wide = w.n_in % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
+  const long long rounded = (units + 31) / 32 * 32;  // whole warps: the lanes of a group meet in the shuffles
+  for (long long u = blockIdx.x * 256LL + threadIdx.x; u < rounded; u += stride) {
+    const bool live = u < units;
+    const long long n = !live ? 0 : units < (1LL << 32) ? (long long)((unsigned)u / per_row) : u / per_row;
+    const int k = live ? (int)(u - n * per_row) * 8 : 0;
+    float v[8];
+    load_eight(W, type, n * w.n_in + k, live ? w.n_in - k : 0, wide, v);
+    uint32_t top = largest(v);
+    for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = __fmul_rn(__uint_as_float(top), 1.f / 7.f);
+    if (live) {
+      reinterpret_cast<uint32_t*>(codes)[u] = codes_of(v, scale, 1.f / scale);
+      if ((threadIdx.x & (lanes - 1)) == 0) scales[(long long)(k >> w.group_log2) * w.n_out + n] = scale;
+    }
+  }
+}
+// Groups over 256: a warp each, which reads it twice.
+__global__ void __launch_bounds__(256) w4_quantise_long_kernel(const void* W, int type, uint8_t* codes, float* scales, W4 w) {
+  const int G = 1 << w.group_log2, lane = threadIdx.x & 31, groups = w.groups();
   const long long units = (long long)w.n_out * groups, stride = (long long)gridDim.x * 8;
+  const bool wide = w.n_in % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
   for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += stride) {
     const long long n = u / groups;
     const int g = (int)(u - n * groups);
     uint32_t top = 0;
-    for (int j = lane; j < G; j += 32) {
-      const int k = g * G + j;
-      if (k < w.n_in) top = max(top, __float_as_uint(load_any(W, type, n * w.n_in + k)) & 0x7fffffffu);
+    float v[8];
+    for (int j = lane * 8; j < G; j += 256) {
+      load_eight(W, type, n * w.n_in + g * G + j, w.n_in - g * G - j, wide, v);
+      top = max(top, largest(v));
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    const float scale = __fmul_rn(__uint_as_float(top), 1.f / 7.f);
+    const float scale = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), 1.f / 7.f);
     if (lane == 0) scales[(long long)g * w.n_out + n] = scale;
-    uint8_t* out = codes + n * w.pitch() + (long long)g * (G / 2);
-    for (int j = lane; j < G / 2; j += 32) {
-      int q[2];
-      for (int h = 0; h < 2; ++h) {
-        const int k = g * G + 2 * j + h;
-        const float v = k < w.n_in ? load_any(W, type, n * w.n_in + k) : 0.f;
-        q[h] = (scale > 0.f && scale < INFINITY) ? min(7, max(-7, __float2int_rn(__fdiv_rn(v, scale)))) : 0;
-      }
-      out[j] = (uint8_t)((q[0] + 8) | ((q[1] + 8) << 4));
+    const float inverse = 1.f / scale;
+    uint32_t* out = reinterpret_cast<uint32_t*>(codes + n * w.pitch() + (long long)g * (G / 2));
+    for (int j = lane * 8; j < G; j += 256) {
+      load_eight(W, type, n * w.n_in + g * G + j, w.n_in - g * G - j, wide, v);
+      out[j / 8] = codes_of(v, scale, inverse);
     }
   }
 }
 
+// code - 8 in 8 bits, or the weight in 32: eight neighbours a thread.
 __global__ void __launch_bounds__(256) w4_unpack_kernel(W4 w, int8_t* integers, float* dense) {
-  const long long total = (long long)w.n_out * w.n_in;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const long long n = i / w.n_in;
-    const int k = (int)(i - n * w.n_in);
-    const int q = ((w.codes[n * w.pitch() + k / 2] >> (4 * (k & 1))) & 15) - 8;
-    if (integers) integers[i] = (int8_t)q;
-    else dense[i] = w.scales[(long long)(k >> w.group_log2) * w.n_out + n] * (float)q;
+  const unsigned per_row = (unsigned)((w.n_in + 7) >> 3);
+  const long long units = (long long)w.n_out * per_row, pitch = w.pitch();
+  for (long long u = blockIdx.x * 256LL + threadIdx.x; u < units; u += gridDim.x * 256LL) {
+    const long long n = units < (1LL << 32) ? (long long)((unsigned)u / per_row) : u / per_row;
+    const int k = (int)(u - n * per_row) * 8, left = min(8, w.n_in - k);
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(w.codes + n * pitch + k / 2);
+    // a byte c of 0..15 to c - 8: (128 + c - 8) with its highest bit turned borrows nothing from its neighbour
+    const uint32_t lo = (((word & 0x0f0f0f0fu) | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
+    const uint32_t hi = ((((word >> 4) & 0x0f0f0f0fu) | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
+    const uint32_t q[2] = {__byte_perm(lo, hi, 0x5140), __byte_perm(lo, hi, 0x7362)};
+    const long long at = n * w.n_in + k;
+    if (integers) {
+      if (w.n_in % 8 == 0 && (reinterpret_cast<uintptr_t>(integers) & 7) == 0) {
+        *reinterpret_cast<uint2*>(integers + at) = make_uint2(q[0], q[1]);
+      } else {
+        for (int j = 0; j < left; ++j) integers[at + j] = (int8_t)(q[j >> 2] >> (8 * (j & 3)));
+      }
+    } else {
+      const float scale = w.scales[(long long)(k >> w.group_log2) * w.n_out + n];
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = scale * (float)(int8_t)(q[j >> 2] >> (8 * (j & 3)));
+      if (w.n_in % 4 == 0 && left == 8 && (reinterpret_cast<uintptr_t>(dense) & 15) == 0) {
+        reinterpret_cast<float4*>(dense + at)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(dense + at)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        for (int j = 0; j < left; ++j) dense[at + j] = v[j];
+      }
+    }
   }
 }
 
@@ -98,7 +192,9 @@ extern "C" int bf_w4_quantise(const void* W, int type, uint8_t* codes, float* sc
   const int rc = bf::make_w4(w, "bf_w4_quantise", codes, scales, n_out, n_in, group);
   if (rc != BF_OK) return rc;
   BF_REQUIRE(W && bf::type_ok(type), BF_E_INVALID, "bf_w4_quantise: null weight or unknown type %d", type);
-  bf::w4_quantise_kernel<<<bf::blocks_for((long long)n_out * w.groups(), 8), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
+  const long long words = (long long)n_out * ((long long)w.groups() << w.group_log2) / 8;
+  if (w.group_log2 <= 8) bf::w4_quantise_kernel<<<bf::blocks_for(words, 256), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
+  else bf::w4_quantise_long_kernel<<<bf::blocks_for((long long)n_out * w.groups(), 8), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
   BF_CHECK_LAUNCH("w4_quantise_kernel");
   return BF_OK;
 }
@@ -108,7 +204,7 @@ extern "C" int bf_w4_integers(const uint8_t* codes, int8_t* out, int n_out, int 
   const int rc = bf::make_w4(w, "bf_w4_integers", codes, codes, n_out, n_in, group);
   if (rc != BF_OK) return rc;
   BF_REQUIRE(out, BF_E_INVALID, "bf_w4_integers: null output");
-  bf::w4_unpack_kernel<<<bf::blocks_for((long long)n_out * n_in, 256), 256, 0, bf::as_stream(stream)>>>(w, out, nullptr);
+  bf::w4_unpack_kernel<<<bf::blocks_for(((long long)n_in + 7) / 8 * n_out, 256), 256, 0, bf::as_stream(stream)>>>(w, out, nullptr);
   BF_CHECK_LAUNCH("w4_unpack_kernel");
   return BF_OK;
 }
@@ -118,7 +214,7 @@ extern "C" int bf_w4_dense(const uint8_t* codes, const float* scales, float* out
   const int rc = bf::make_w4(w, "bf_w4_dense", codes, scales, n_out, n_in, group);
   if (rc != BF_OK) return rc;
   BF_REQUIRE(out, BF_E_INVALID, "bf_w4_dense: null output");
-  bf::w4_unpack_kernel<<<bf::blocks_for((long long)n_out * n_in, 256), 256, 0, bf::as_stream(stream)>>>(w, nullptr, out);
+  bf::w4_unpack_kernel<<<bf::blocks_for(((long long)n_in + 7) / 8 * n_out, 256), 256, 0, bf::as_stream(stream)>>>(w, nullptr, out);
   BF_CHECK_LAUNCH("w4_unpack_kernel");
   return BF_OK;
 }

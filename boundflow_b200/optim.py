@@ -6,15 +6,20 @@ runtime/alpha_beta_crown.py:747-923).  `AdamW` is the step for the network's own
 """
 from __future__ import annotations
 
+import operator
 from typing import Any, Dict, Iterable, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from . import _lib
-from .network import _stream_ptr
+from .weights4 import _Entry
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
+_PAIRS = {(p, g) for p in _TYPES for g in _TYPES if p == g or p == torch.float32}
+_GRAD, _SHAPE, _DEVICE, _LAYOUT, _DTYPE = (operator.attrgetter(n) for n in ("grad", "shape", "device", "layout", "dtype"))
+_POINTER, _NUMEL, _CONTIGUOUS = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_ADAMW_STEP, _ADAMW_MOMENTS = _Entry("bf_adamw_step"), _Entry("bf_adamw_moments")
 _BLOCK = 256  # moments that share an exponent; a tensor's moments begin at a whole block
 _ENTRY = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.int64), ("first", np.int64), ("lr", np.float32), ("weight_decay", np.float32)])
 
@@ -66,6 +71,7 @@ class AdamW:
         self._options()
         self.betas, self.eps, self.state_bits, self.device = (b1, b2), float(eps), state_bits, self._params[0].device
         self._sizes = [p.numel() for p in self._params]
+        self._inference = any(p.is_inference() for p in self._params)
         self._first = np.concatenate([[0], np.cumsum([-(-n // _BLOCK) * _BLOCK for n in self._sizes])]).astype(np.int64)
         total = max(_BLOCK, int(self._first[-1]))
         kind = torch.float32 if state_bits == 32 else torch.uint8
@@ -103,7 +109,7 @@ class AdamW:
         """One step with the tensors' `.grad`, or with `grads` (one for each tensor, in order; None leaves that one as it is).  `grad_scale`: a device
         tensor of one fp32 element that the gradients are multiplied by (a clip factor, one over a loss scale)."""
         params, device = self._params, self.device
-        given = [p.grad for p in params] if grads is None else list(grads)
+        given = list(map(_GRAD, params)) if grads is None else list(grads)
         if len(given) != len(params):
             raise ValueError(f"AdamW.step: {len(given)} gradients for {len(params)} tensors")
         scale = None
@@ -112,39 +118,43 @@ class AdamW:
                 raise ValueError(f"AdamW.step: grad_scale is one fp32 element on {device}")
             scale = grad_scale.data_ptr()
         lr, decay = self._options()
-        buckets: Dict[Tuple[torch.dtype, torch.dtype], List[int]] = {}
-        kept = []  # copies that live until the launch
-        pointers = [0] * len(params)
-        for k, (p, g) in enumerate(zip(params, given)):
-            if g is None:
-                continue
-            if g.dtype != p.dtype and (p.dtype != torch.float32 or g.dtype not in _TYPES):
-                raise TypeError(f"AdamW.step: gradient {k} is {g.dtype} for a tensor of {p.dtype}")
-            if g.shape != p.shape or g.device != device or g.layout != torch.strided:
-                raise ValueError(f"AdamW.step: gradient {k} is {tuple(g.shape)} on {g.device} for a tensor {tuple(p.shape)} on {device}")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept.append(g)
-            if not p.is_contiguous() or p.numel() != self._sizes[k]:
-                raise ValueError(f"AdamW.step: tensor {k} has changed its shape or strides")
-            pointers[k] = g.data_ptr()
-            buckets.setdefault((p.dtype, g.dtype), []).append(k)
-        if not buckets:
-            return
-        table = self._table
-        table["p"], table["g"] = [p.data_ptr() for p in params], pointers
-        for i in range(len(lr)):
-            at = slice(None) if len(lr) == 1 else [k for k, j in enumerate(self._group_of) if j == i]
-            table["lr"][at], table["weight_decay"][at] = lr[i], decay[i]
-        lib = _lib.load()
-        with torch.cuda.device(device):
-            stream = _stream_ptr(device)
-            for n, ((pt, gt), at) in enumerate(buckets.items()):
-                part = table if len(at) == len(params) else np.ascontiguousarray(table[at])
-                _lib.check(lib.bf_adamw_step(part.ctypes.data, len(at), _TYPES[pt], _TYPES[gt], self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                                             _lib.ptr(self.exp_avg_exponent), _lib.ptr(self.exp_avg_sq_exponent), self.betas[0], self.betas[1], self.eps, scale,
-                                             self._state.data_ptr(), 1 if n + 1 == len(buckets) else 0, stream))
-        torch.autograd.graph.increment_version([p for p, g in zip(params, given) if g is not None and not p.is_inference()])
+        live = range(len(params))
+        moved = params
+        if any(g is None for g in given):
+            live = [k for k, g in enumerate(given) if g is not None]
+            if not live:
+                return
+            moved, given = [params[k] for k in live], [given[k] for k in live]
+        if grads is not None:  # (a tensor's .grad has its shape, type and device)
+            shapes = list(map(_SHAPE, moved))
+            if list(map(_SHAPE, given)) != shapes or set(map(_DEVICE, given)) != {device}:
+                k = next(k for k, g, s in zip(live, given, shapes) if g.shape != s or g.device != device)
+                raise ValueError(f"AdamW.step: gradient {k} is {tuple(given[list(live).index(k)].shape)} on {given[list(live).index(k)].device}, not "
+                                 f"{tuple(params[k].shape)} on {device}")
+        if set(map(_LAYOUT, given)) != {torch.strided}:
+            raise ValueError("AdamW.step: gradients have to be strided tensors")
+        sizes = self._sizes if moved is params else [self._sizes[k] for k in live]
+        if list(map(_NUMEL, moved)) != sizes or list(map(_NUMEL, given)) != sizes or not all(map(_CONTIGUOUS, moved)):
+            raise ValueError("AdamW.step: a tensor has changed its shape or strides")
+        if not all(map(_CONTIGUOUS, given)):
+            given = [g.contiguous() for g in given]  # (copies live until the launch)
+        kinds = list(zip(map(_DTYPE, moved), map(_DTYPE, given)))
+        for k, (pt, gt) in zip(live, kinds) if len(set(kinds)) > 1 or kinds[0] not in _PAIRS else ():
+            if (pt, gt) not in _PAIRS:
+                raise TypeError(f"AdamW.step: gradient {k} is {gt} for a tensor of {pt}")
+        table = self._table if moved is params else self._table[live]
+        table["p"], table["g"] = list(map(_POINTER, moved)), list(map(_POINTER, given))
+        if len(lr) == 1:
+            table["lr"], table["weight_decay"] = lr[0], decay[0]
+        else:
+            table["lr"], table["weight_decay"] = [lr[self._group_of[k]] for k in live], [decay[self._group_of[k]] for k in live]
+        buckets = [(kinds[0], table)] if kinds.count(kinds[0]) == len(kinds) else \
+            [(kind, np.ascontiguousarray(table[[i for i, other in enumerate(kinds) if other == kind]])) for kind in dict.fromkeys(kinds)]
+        for n, ((pt, gt), part) in enumerate(buckets):
+            _ADAMW_STEP(device, part.ctypes.data, len(part), _TYPES[pt], _TYPES[gt], self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                        _lib.ptr(self.exp_avg_exponent), _lib.ptr(self.exp_avg_sq_exponent), self.betas[0], self.betas[1], self.eps, scale,
+                        self._state.data_ptr(), 1 if n + 1 == len(buckets) else 0)
+        torch.autograd.graph.increment_version(moved if not self._inference else [p for p in moved if not p.is_inference()])
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for p in self._params:
@@ -166,9 +176,8 @@ class AdamW:
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
         m, v = (torch.empty(self.exp_avg.numel(), dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().bf_adamw_moments(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_exponent.data_ptr(),
-                                                    self.exp_avg_sq_exponent.data_ptr(), m.data_ptr(), v.data_ptr(), m.numel(), _stream_ptr(self.device)))
+        _ADAMW_MOMENTS(self.device, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_exponent.data_ptr(), self.exp_avg_sq_exponent.data_ptr(),
+                       m.data_ptr(), v.data_ptr(), m.numel())
         return m, v
 
     @property

@@ -20,7 +20,7 @@ from typing import Any, Optional, Tuple
 import torch
 
 from . import _lib
-from .network import _cuda_device, _stream_ptr
+from .network import _cuda_device
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 
@@ -64,16 +64,14 @@ class Weight4:
         return 2
 
     def to(self, device: Any) -> "Weight4":
-        device = torch.device(device)
-        return self if device == self.device else Weight4(self.codes.to(device), self.scales.to(device), self.n_in)
+        return self if self.codes.device == (device if isinstance(device, torch.device) else torch.device(device)) else Weight4(self.codes.to(device), self.scales.to(device), self.n_in)
 
     def integers(self) -> torch.Tensor:
         """code - 8 as int8 [n_out, n_in]."""
         device = _device_of(self.codes)
         w = self.to(device)
         out = torch.empty(w.shape, dtype=torch.int8, device=device)
-        with torch.cuda.device(device):
-            _lib.check(_lib.load().bf_w4_integers(w.codes.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group, _stream_ptr(device)))
+        _W4_INTEGERS(device, w.codes.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group)
         return out.to(self.device)
 
     def dense(self) -> torch.Tensor:
@@ -81,8 +79,7 @@ class Weight4:
         device = _device_of(self.codes)
         w = self.to(device)
         out = torch.empty(w.shape, dtype=torch.float32, device=device)
-        with torch.cuda.device(device):
-            _lib.check(_lib.load().bf_w4_dense(w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group, _stream_ptr(device)))
+        _W4_DENSE(device, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group)
         return out.to(self.device)
 
     def __repr__(self) -> str:
@@ -109,49 +106,69 @@ def quantise_weight4(W: torch.Tensor, group: int = 128) -> Weight4:
     groups = -(-n_in // group)
     codes = torch.empty(n_out, groups * group // 2, dtype=torch.uint8, device=device)
     scales = torch.empty(groups, n_out, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().bf_w4_quantise(w.data_ptr(), _TYPES[w.dtype], codes.data_ptr(), scales.data_ptr(), n_out, n_in, group, _stream_ptr(device)))
+    _W4_QUANTISE(device, w.data_ptr(), _TYPES[w.dtype], codes.data_ptr(), scales.data_ptr(), n_out, n_in, group)
     return Weight4(codes, scales, n_in).to(W.device)
 
 
 # ---- launches: contiguous CUDA tensors of one device, rows [M, n] -----------------------
+class _Entry:
+    """An entry point of the library, called with the tensors' device current.  (torch.cuda.device and the arity check cost a call of few microseconds more than its
+    kernel takes; the argument lists below are fixed.)"""
+
+    def __init__(self, name: str):
+        self.name, self.fn = name, None
+
+    def __call__(self, device: torch.device, *args) -> None:
+        fn = self.fn
+        if fn is None:
+            fn = self.fn = getattr(_lib.load(), self.name).unchecked
+        index = device.index
+        before = torch._C._cuda_getDevice()
+        if before == index:
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(device):
+                code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if code:
+            _lib.check(code)
+
+
+_W4_LINEAR, _W4_INTERVAL, _W4_ROWS, _W4_INTERVAL_GRAD = (_Entry(n) for n in ("bf_w4_linear", "bf_w4_interval", "bf_w4_rows", "bf_w4_interval_grad"))
+_W4_QUANTISE, _W4_INTEGERS, _W4_DENSE, _COLUMN_SUMS = (_Entry(n) for n in ("bf_w4_quantise", "bf_w4_integers", "bf_w4_dense", "bf_column_sums"))
+
+
 def _linear(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor]) -> torch.Tensor:
-    M, device = int(x.shape[0]), x.device
-    y = torch.empty(M, w.n_out, dtype=x.dtype, device=device)
+    M = x.shape[0]
+    y = x.new_empty((M, w.n_out))
     if M:
-        with torch.cuda.device(device):
-            _lib.check(_lib.load().bf_w4_linear(x.data_ptr(), _TYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), _lib.ptr(bias),
-                                                _TYPES[bias.dtype] if bias is not None else 0, y.data_ptr(), M, w.n_in, w.n_out, w.group, _stream_ptr(device)))
+        _W4_LINEAR(x.device, x.data_ptr(), _TYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                   0 if bias is None else _TYPES[bias.dtype], y.data_ptr(), M, w.n_in, w.n_out, w.group)
     return y
 
 
 def _interval(a: torch.Tensor, b: torch.Tensor, mode: int, relu_in: int, w: Weight4, bias: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    M, device = int(a.shape[0]), a.device
-    lower, upper = (torch.empty(M, w.n_out, dtype=torch.float32, device=device) for _ in range(2))
+    M = a.shape[0]
+    lower, upper = a.new_empty((M, w.n_out)), a.new_empty((M, w.n_out))
     if M:
-        with torch.cuda.device(device):
-            _lib.check(_lib.load().bf_w4_interval(a.data_ptr(), b.data_ptr(), mode, relu_in, w.codes.data_ptr(), w.scales.data_ptr(), _lib.ptr(bias), lower.data_ptr(),
-                                                  upper.data_ptr(), M, w.n_in, w.n_out, w.group, _stream_ptr(device)))
+        _W4_INTERVAL(a.device, a.data_ptr(), b.data_ptr(), mode, relu_in, w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                     lower.data_ptr(), upper.data_ptr(), M, w.n_in, w.n_out, w.group)
     return lower, upper
 
 
 def _rows(a: torch.Tensor, w: Weight4) -> torch.Tensor:
-    M, device = int(a.shape[0]), a.device
-    z = torch.empty(M, w.n_in, dtype=a.dtype, device=device)
+    M = a.shape[0]
+    z = a.new_empty((M, w.n_in))
     if M:
-        with torch.cuda.device(device):
-            _lib.check(_lib.load().bf_w4_rows(a.data_ptr(), _TYPES[a.dtype], w.codes.data_ptr(), w.scales.data_ptr(), z.data_ptr(), M, w.n_in, w.n_out, w.group,
-                                              _stream_ptr(device)))
+        _W4_ROWS(a.device, a.data_ptr(), _TYPES[a.dtype], w.codes.data_ptr(), w.scales.data_ptr(), z.data_ptr(), M, w.n_in, w.n_out, w.group)
     return z
 
 
 def _column_sums(a: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    M, n, device = int(a.shape[0]), int(a.shape[1]), a.device
+    M, n = a.shape
     if M == 0:
-        return torch.zeros(n, dtype=dtype, device=device)
-    out = torch.empty(n, dtype=dtype, device=device)
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().bf_column_sums(a.data_ptr(), _TYPES[a.dtype], out.data_ptr(), _TYPES[dtype], M, n, _stream_ptr(device)))
+        return a.new_zeros(n, dtype=dtype)
+    out = a.new_empty(n, dtype=dtype)
+    _COLUMN_SUMS(a.device, a.data_ptr(), _TYPES[a.dtype], out.data_ptr(), _TYPES[dtype], M, n)
     return out
 
 
@@ -162,12 +179,26 @@ class _Linear4(torch.autograd.Function):
         return _linear(x, weight, bias)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        again = dy.requires_grad and torch.is_grad_enabled()  # a gradient of this gradient is asked for
         dy = dy.contiguous()
-        dx = _rows(dy, ctx.weight) if ctx.needs_input_grad[0] else None
-        db = _column_sums(dy, ctx.bias_type) if ctx.needs_input_grad[1] else None
+        dx = (_Rows4.apply(dy, ctx.weight) if again else _rows(dy, ctx.weight)) if need[0] else None
+        db = (dy.float().sum(0).to(ctx.bias_type) if again else _column_sums(dy, ctx.bias_type)) if need[1] else None
         return dx, db, None
+
+
+class _Rows4(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, weight):
+        ctx.weight = weight
+        return _rows(a, weight)
+
+    @staticmethod
+    def backward(ctx, dz):
+        again = dz.requires_grad and torch.is_grad_enabled()
+        dz = dz.contiguous()
+        return (_Linear4.apply(dz, None, ctx.weight) if again else _linear(dz, ctx.weight, None)), None
 
 
 class _Interval4(torch.autograd.Function):
@@ -179,16 +210,14 @@ class _Interval4(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dl, du):
-        w, device = ctx.weight, dl.device
+        w = ctx.weight
         dl, du = dl.contiguous(), du.contiguous()
-        M = int(dl.shape[0])
+        M = dl.shape[0]
         gl = gu = db = None
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            gl, gu = (torch.empty(M, w.n_in, dtype=torch.float32, device=device) for _ in range(2))
+            gl, gu = dl.new_empty((M, w.n_in)), dl.new_empty((M, w.n_in))
             if M:
-                with torch.cuda.device(device):
-                    _lib.check(_lib.load().bf_w4_interval_grad(dl.data_ptr(), du.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gl.data_ptr(), gu.data_ptr(),
-                                                               M, w.n_in, w.n_out, w.group, _stream_ptr(device)))
+                _W4_INTERVAL_GRAD(dl.device, dl.data_ptr(), du.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gl.data_ptr(), gu.data_ptr(), M, w.n_in, w.n_out, w.group)
         if ctx.needs_input_grad[2]:
             db = _column_sums(dl, torch.float32) + _column_sums(du, torch.float32)
         return gl, gu, db, None
@@ -199,37 +228,37 @@ def _check_rows(name: str, x: Any, weight: Any, width: str) -> None:
         raise TypeError(f"{name}: the weight is a Weight4 (quantise_weight4 makes one), got {type(weight)}")
     if not torch.is_tensor(x) or x.dtype not in _TYPES:
         raise TypeError(f"{name} takes fp32, bf16 or fp16 tensors")
-    if x.dim() < 1 or int(x.shape[-1]) != getattr(weight, width):
+    if x.dim() < 1 or x.shape[-1] != getattr(weight, width):
         raise ValueError(f"{name}: rows of {int(x.shape[-1]) if x.dim() else 0} do not match {weight!r}")
 
 
 def _check_bias(name: str, bias: Any, weight: Weight4) -> None:
     if bias is not None and (not torch.is_tensor(bias) or bias.dtype not in _TYPES):
         raise TypeError(f"{name} takes an fp32, bf16 or fp16 bias")
-    if bias is not None and tuple(bias.shape) != (weight.n_out,):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != weight.n_out):
         raise ValueError(f"{name}: bias {tuple(bias.shape)} does not match {weight!r}")
 
 
-def _at(t: Optional[torch.Tensor], device: torch.device) -> Optional[torch.Tensor]:
-    return t if t is None or t.device == device else t.to(device)
+def _placed(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """`t` on `device`, contiguous: itself where it is so already."""
+    return t if t.is_cuda and t.device == device and t.is_contiguous() else t.to(device).contiguous()
 
 
 def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable once, for x and bias."""
+    """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable in x and bias."""
     _check_rows("linear4", x, weight, "n_in")
     _check_bias("linear4", bias, weight)
     device = _device_of(x)
-    w, b = weight.to(device), _at(bias, device)
-    rows = _at(x, device).reshape(-1, weight.n_in).contiguous()
-    if b is not None:
-        b = b.contiguous()
+    w, b = weight.to(device), bias if bias is None else _placed(bias, device)
+    flat = x.dim() == 2
+    rows = _placed(x if flat else x.reshape(-1, weight.n_in), device)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         y = _Linear4.apply(rows, b, w)
     else:
         y = _linear(rows, w, b)
-    if x.dim() != 2:
+    if not flat:
         y = y.reshape(x.shape[:-1] + (weight.n_out,))
-    return y if y.device == x.device else y.to(x.device)
+    return y if x.is_cuda else y.to(x.device)
 
 
 def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None, *,
@@ -244,29 +273,28 @@ def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, 
     if lower.dtype != torch.float32 or upper.dtype != torch.float32 or (bias is not None and bias.dtype != torch.float32):
         raise TypeError("interval_linear4 takes fp32: bounds rounded to 16 bits would not hold")
     device = _device_of(lower)
-    w, b = weight.to(device), _at(bias, device)
-    lo, up = (_at(t, device).reshape(-1, weight.n_in).contiguous() for t in (lower, upper))
-    if b is not None:
-        b = b.contiguous()
+    w, b = weight.to(device), bias if bias is None else _placed(bias, device)
+    flat = lower.dim() == 2
+    lo, up = (_placed(t if flat else t.reshape(-1, weight.n_in), device) for t in (lower, upper))
     if torch.is_grad_enabled() and (lower.requires_grad or upper.requires_grad or (bias is not None and bias.requires_grad)):
         if relu_in:
             raise NotImplementedError("interval_linear4 has no gradient with relu_in; clamp the bounds before the call")
         yl, yu = _Interval4.apply(lo, up, b, w)
     else:
         yl, yu = _interval(lo, up, _lib.IN_LOWER_UPPER, 1 if relu_in else 0, w, b)
-    if lower.dim() != 2:
+    if not flat:
         shape = lower.shape[:-1] + (weight.n_out,)
         yl, yu = yl.reshape(shape), yu.reshape(shape)
-    return (yl, yu) if yl.device == lower.device else (yl.to(lower.device), yu.to(lower.device))
+    return (yl, yu) if lower.is_cuda else (yl.to(lower.device), yu.to(lower.device))
 
 
 def rows_times_weight4(A: torch.Tensor, weight: Weight4) -> torch.Tensor:
-    """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once).  No gradient: it is one, of `linear4`."""
+    """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once): the gradient of `linear4`.  Differentiable in A."""
     _check_rows("rows_times_weight4", A, weight, "n_out")
-    if torch.is_grad_enabled() and A.requires_grad:
-        raise NotImplementedError("rows_times_weight4 has no gradient; detach the rows")
     device = _device_of(A)
-    z = _rows(_at(A, device).reshape(-1, weight.n_out).contiguous(), weight.to(device))
-    if A.dim() != 2:
+    flat = A.dim() == 2
+    rows, w = _placed(A if flat else A.reshape(-1, weight.n_out), device), weight.to(device)
+    z = _Rows4.apply(rows, w) if A.requires_grad and torch.is_grad_enabled() else _rows(rows, w)
+    if not flat:
         z = z.reshape(A.shape[:-1] + (weight.n_in,))
-    return z if z.device == A.device else z.to(A.device)
+    return z if A.is_cuda else z.to(A.device)

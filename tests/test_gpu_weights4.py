@@ -114,6 +114,21 @@ def test_linear_gradients(dev, kind, m, n, k, group):
     check(gb, d.sum((0, 1)), d.abs().sum((0, 1)), 2 * m * 8, b.dtype)
 
 
+def test_gradients_of_gradients(dev):
+    """d / d dy of (dx . v) is v W^T, and d / d a of (a W . v) the same: products with the weight again."""
+    from boundflow_b200.weights4 import linear4, rows_times_weight4
+
+    W, w, g = make(70, 90, 32, dev, 8)
+    x, b = torch.randn(3, 90, generator=g).to(dev).requires_grad_(), torch.randn(70, generator=g).to(dev).requires_grad_()
+    dy, v, u = torch.randn(3, 70, generator=g).to(dev).requires_grad_(), torch.randn(3, 90, generator=g).to(dev), torch.randn(70, generator=g).to(dev)
+    gx, gb = torch.autograd.grad(linear4(x, W, b), (x, b), dy, create_graph=True)
+    got, = torch.autograd.grad((gx, gb), dy, (v, u))
+    check(got, v.double() @ w.t() + u.double(), v.double().abs() @ w.abs().t() + u.double().abs(), 90, torch.float32)
+    a = torch.randn(2, 2, 70, generator=g).to(dev).requires_grad_()
+    got, = torch.autograd.grad(rows_times_weight4(a, W), a, v[:2].expand(2, 2, 90))
+    check(got, (v[:2].double() @ w.t()).expand(2, 2, 70), (v[:2].double().abs() @ w.abs().t()).expand(2, 2, 70), 90, torch.float32)
+
+
 @pytest.mark.parametrize("m,n,k,group", [(1, 7, 40, 32), (4, 130, 300, 64), (19, 65, 129, 128)])
 def test_interval_gradients(dev, m, n, k, group):
     """Against the formula and against differences: the bounds are linear in lower and upper while W keeps its signs, so a difference of any length is exact."""
