@@ -36,50 +36,85 @@ __device__ __forceinline__ uint32_t largest(const float (&v)[8]) {
   }
   return finite == 0.f ? __float_as_uint(top) : 0x7fc00000u;
 }
-// Eight codes.  The quotient is the rounded one of a division by definition; a product with the reciprocal is within 2^-20 of it, so that both round to the same
-// whole number unless they lie that near to half of one: those are divided.  Adding 1.5 * 2^23 rounds to a whole number and leaves it, + 8, in the last bits, which
-// are collected with products: what the sum of the constants' own bits comes to is taken off at the end.
+// Eight codes.  The quotient is the rounded one of a division by definition: with the rounded reciprocal, a product and the remainder that it leaves give it exactly
+// (Markstein 1990).  Adding 1.5 * 2^23 rounds to a whole number and leaves it, + 8, in the last bits, which are collected with products: what the
+// constants' own bits come to is taken off at the end.  (16-bit weights lie on a lattice, halves of a code are frequent among them: no branch for those.)
 __device__ __forceinline__ uint32_t codes_of(const float (&v)[8], float scale, float inverse) {
-  constexpr float MAGIC = 12582912.f + 8.f;
   if (!(scale > 0.f && scale < INFINITY)) return 0x88888888u;  // zeros, or a group that its scale makes NaN
-  float off = inverse < INFINITY ? 0.f : 1.f;
   uint32_t word = 0;
+  if (scale > 1e-30f) {
 #pragma unroll
-  for (int j = 7; j >= 0; --j) {
-    const float t = fmaf(v[j], inverse, MAGIC);
-    off = fmaxf(off, fabsf(fmaf(v[j], inverse, MAGIC - t)));
-    word = word * 16u + __float_as_uint(t);
+    for (int j = 7; j >= 0; --j) {
+      const float near = v[j] * inverse;
+      word = word * 16u + __float_as_uint(fmaf(fmaf(-near, scale, v[j]), inverse, near) + (12582912.f + 8.f));
+    }
+    return word - 0x4B400000u * 0x11111111u;
   }
-  if (off > 0.49999f) {
-    word = 0;
 #pragma unroll
-    for (int j = 7; j >= 0; --j) word = word * 16u + (uint32_t)(__float2int_rn(fminf(fmaxf(rintf(__fdiv_rn(v[j], scale)), -7.f), 7.f)) + 8);
-    return word;
-  }
-  return word - 0x4B400000u * 0x11111111u;
+  for (int j = 7; j >= 0; --j) word = word * 16u + (uint32_t)(__float2int_rn(fminf(fmaxf(rintf(__fdiv_rn(v[j], scale)), -7.f), 7.f)) + 8);
+  return word;
 }
 
 // Largest magnitude of a group, scale = that times 1/7 (as a 32-bit number), codes = round(w / scale) + 8.  The largest is taken over bit patterns, whose order
 // is that of the magnitudes with infinities and NaN above: a group that holds one has it as its scale and is NaN throughout.
 // A thread takes eight neighbours; as many lanes as a group of up to 256 needs share its largest (groups do not straddle warps).
-__global__ void __launch_bounds__(256) w4_quantise_kernel(const void* W, int type, uint8_t* codes, float* scales, W4 w) {
-  const unsigned per_row = (unsigned)((w.groups() << w.group_log2) >> 3);
-  const int lanes = 1 << (w.group_log2 - 3);
-  const long long units = (long long)w.n_out * per_row, stride = (long long)gridDim.x * 256;
+// A warp's turn is 1024 columns of a row, all on their way before the first are worked on.
+template <typename T> struct Raw { uint4 q; };
+template <> struct Raw<float> { uint4 q, r; };
+__device__ __forceinline__ void numbers(const Raw<float>& w, float (&v)[8]) {
+  const uint32_t q[8] = {w.q.x, w.q.y, w.q.z, w.q.w, w.r.x, w.r.y, w.r.z, w.r.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(q[j]);
+}
+__device__ __forceinline__ void numbers(const Raw<__nv_bfloat16>& w, float (&v)[8]) {
+  const uint32_t q[4] = {w.q.x, w.q.y, w.q.z, w.q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(q[j] << 16);
+    v[2 * j + 1] = __uint_as_float(q[j] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void numbers(const Raw<__half>& w, float (&v)[8]) {
+  const uint32_t q[4] = {w.q.x, w.q.y, w.q.z, w.q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) w4_quantise_kernel(const T* W, int type, uint8_t* codes, float* scales, W4 w) {
+  constexpr int AHEAD = 4;
+  const int padded = w.groups() << w.group_log2, lane8 = (threadIdx.x & 31) * 8, lanes = 1 << (w.group_log2 - 3);
+  const unsigned per_row = (unsigned)(padded + 1023) >> 10;
+  const long long turns = (long long)w.n_out * per_row, stride = (long long)gridDim.x * 8;
   const bool wide = w.n_in % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
-  const long long rounded = (units + 31) / 32 * 32;  // whole warps: the lanes of a group meet in the shuffles
-  for (long long u = blockIdx.x * 256LL + threadIdx.x; u < rounded; u += stride) {
-    const bool live = u < units;
-    const long long n = !live ? 0 : units < (1LL << 32) ? (long long)((unsigned)u / per_row) : u / per_row;
-    const int k = live ? (int)(u - n * per_row) * 8 : 0;
-    float v[8];
-    load_eight(W, type, n * w.n_in + k, live ? w.n_in - k : 0, wide, v);
-    uint32_t top = largest(v);
-    for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = __fmul_rn(__uint_as_float(top), 1.f / 7.f);
-    if (live) {
-      reinterpret_cast<uint32_t*>(codes)[u] = codes_of(v, scale, 1.f / scale);
-      if ((threadIdx.x & (lanes - 1)) == 0) scales[(long long)(k >> w.group_log2) * w.n_out + n] = scale;
+  for (long long turn = blockIdx.x * 8LL + (threadIdx.x >> 5); turn < turns; turn += stride) {
+    const long long n = per_row == 1 ? turn : turns < (1LL << 32) ? (long long)((unsigned)turn / per_row) : turn / per_row;
+    const int k0 = (int)(turn - n * per_row) * 1024 + lane8;
+    const T* from = W + n * w.n_in + k0;
+    uint32_t* out = reinterpret_cast<uint32_t*>(codes + (n * padded + k0) / 2);
+    float* to = scales + (long long)(k0 >> w.group_log2) * w.n_out + n;
+    const bool whole = wide && k0 - lane8 + 256 * AHEAD <= w.n_in;
+    Raw<T> raw[AHEAD];
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) raw[i] = *reinterpret_cast<const Raw<T>*>(from + 256 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (k0 - lane8 + 256 * i >= padded) break;  // (for the whole warp: the lanes of a group meet in the shuffles)
+      float v[8];
+      if (whole) numbers(raw[i], v);
+      else load_eight(W, type, n * w.n_in + k0 + 256 * i, w.n_in - k0 - 256 * i, wide, v);
+      uint32_t top = largest(v);
+      for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float scale = __fmul_rn(__uint_as_float(top), 1.f / 7.f);
+      if (k0 + 256 * i < padded) {
+        out[32 * i] = codes_of(v, scale, __frcp_rn(scale));
+        if ((threadIdx.x & (lanes - 1)) == 0) to[(long long)((256 * i) >> w.group_log2) * w.n_out] = scale;
+      }
     }
   }
 }
@@ -99,7 +134,7 @@ __global__ void __launch_bounds__(256) w4_quantise_long_kernel(const void* W, in
     }
     const float scale = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), 1.f / 7.f);
     if (lane == 0) scales[(long long)g * w.n_out + n] = scale;
-    const float inverse = 1.f / scale;
+    const float inverse = __frcp_rn(scale);
     uint32_t* out = reinterpret_cast<uint32_t*>(codes + n * w.pitch() + (long long)g * (G / 2));
     for (int j = lane * 8; j < G; j += 256) {
       load_eight(W, type, n * w.n_in + g * G + j, w.n_in - g * G - j, wide, v);
@@ -192,9 +227,13 @@ extern "C" int bf_w4_quantise(const void* W, int type, uint8_t* codes, float* sc
   const int rc = bf::make_w4(w, "bf_w4_quantise", codes, scales, n_out, n_in, group);
   if (rc != BF_OK) return rc;
   BF_REQUIRE(W && bf::type_ok(type), BF_E_INVALID, "bf_w4_quantise: null weight or unknown type %d", type);
-  const long long words = (long long)n_out * ((long long)w.groups() << w.group_log2) / 8;
-  if (w.group_log2 <= 8) bf::w4_quantise_kernel<<<bf::blocks_for(words, 256), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
-  else bf::w4_quantise_long_kernel<<<bf::blocks_for((long long)n_out * w.groups(), 8), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
+  const long long turns = (long long)n_out * ((((long long)w.groups() << w.group_log2) + 1023) / 1024);
+  if (w.group_log2 <= 8) {
+    const int blocks = bf::blocks_for(turns, 8);
+    if (type == BF_TYPE_F32) bf::w4_quantise_kernel<<<blocks, 256, 0, bf::as_stream(stream)>>>(static_cast<const float*>(W), type, codes, scales, w);
+    else if (type == BF_TYPE_BF16) bf::w4_quantise_kernel<<<blocks, 256, 0, bf::as_stream(stream)>>>(static_cast<const __nv_bfloat16*>(W), type, codes, scales, w);
+    else bf::w4_quantise_kernel<<<blocks, 256, 0, bf::as_stream(stream)>>>(static_cast<const __half*>(W), type, codes, scales, w);
+  } else bf::w4_quantise_long_kernel<<<bf::blocks_for((long long)n_out * w.groups(), 8), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
   BF_CHECK_LAUNCH("w4_quantise_kernel");
   return BF_OK;
 }

@@ -6,6 +6,8 @@ runtime/alpha_beta_crown.py:747-923).  `AdamW` is the step for the network's own
 """
 from __future__ import annotations
 
+import array
+import itertools
 import operator
 from typing import Any, Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -17,8 +19,9 @@ from .weights4 import _Entry
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 _PAIRS = {(p, g) for p in _TYPES for g in _TYPES if p == g or p == torch.float32}
-_GRAD, _SHAPE, _DEVICE, _LAYOUT, _DTYPE = (operator.attrgetter(n) for n in ("grad", "shape", "device", "layout", "dtype"))
-_POINTER, _NUMEL, _CONTIGUOUS = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_SIZE = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}
+_GRAD, _SHAPE, _DEVICE, _DTYPE, _BYTES = (operator.attrgetter(n) for n in ("grad", "shape", "device", "dtype", "nbytes"))
+_POINTER, _CONTIGUOUS = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 _ADAMW_STEP, _ADAMW_MOMENTS = _Entry("bf_adamw_step"), _Entry("bf_adamw_moments")
 _BLOCK = 256  # moments that share an exponent; a tensor's moments begin at a whole block
 _ENTRY = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.int64), ("first", np.int64), ("lr", np.float32), ("weight_decay", np.float32)])
@@ -70,7 +73,7 @@ class AdamW:
         self._refuse_overlap()
         self._options()
         self.betas, self.eps, self.state_bits, self.device = (b1, b2), float(eps), state_bits, self._params[0].device
-        self._sizes = [p.numel() for p in self._params]
+        self._sizes, self._types = [p.numel() for p in self._params], [p.dtype for p in self._params]
         self._inference = any(p.is_inference() for p in self._params)
         self._first = np.concatenate([[0], np.cumsum([-(-n // _BLOCK) * _BLOCK for n in self._sizes])]).astype(np.int64)
         total = max(_BLOCK, int(self._first[-1]))
@@ -118,42 +121,41 @@ class AdamW:
                 raise ValueError(f"AdamW.step: grad_scale is one fp32 element on {device}")
             scale = grad_scale.data_ptr()
         lr, decay = self._options()
-        live = range(len(params))
-        moved = params
-        if any(g is None for g in given):
+        live, moved, sizes, ptypes = range(len(params)), params, self._sizes, self._types
+        if any(map(operator.is_, given, itertools.repeat(None))):
             live = [k for k, g in enumerate(given) if g is not None]
             if not live:
                 return
-            moved, given = [params[k] for k in live], [given[k] for k in live]
+            moved, given, sizes, ptypes = ([xs[k] for k in live] for xs in (params, given, sizes, ptypes))
         if grads is not None:  # (a tensor's .grad has its shape, type and device)
             shapes = list(map(_SHAPE, moved))
             if list(map(_SHAPE, given)) != shapes or set(map(_DEVICE, given)) != {device}:
-                k = next(k for k, g, s in zip(live, given, shapes) if g.shape != s or g.device != device)
-                raise ValueError(f"AdamW.step: gradient {k} is {tuple(given[list(live).index(k)].shape)} on {given[list(live).index(k)].device}, not "
-                                 f"{tuple(params[k].shape)} on {device}")
-        if set(map(_LAYOUT, given)) != {torch.strided}:
-            raise ValueError("AdamW.step: gradients have to be strided tensors")
-        sizes = self._sizes if moved is params else [self._sizes[k] for k in live]
-        if list(map(_NUMEL, moved)) != sizes or list(map(_NUMEL, given)) != sizes or not all(map(_CONTIGUOUS, moved)):
-            raise ValueError("AdamW.step: a tensor has changed its shape or strides")
+                k, g = next((k, g) for k, g, s in zip(live, given, shapes) if g.shape != s or g.device != device)
+                raise ValueError(f"AdamW.step: gradient {k} is {tuple(g.shape)} on {g.device}, not {tuple(params[k].shape)} on {device}")
         if not all(map(_CONTIGUOUS, given)):
+            if any(g.layout is not torch.strided for g in given):
+                raise ValueError("AdamW.step: gradients have to be strided tensors")
             given = [g.contiguous() for g in given]  # (copies live until the launch)
-        kinds = list(zip(map(_DTYPE, moved), map(_DTYPE, given)))
-        for k, (pt, gt) in zip(live, kinds) if len(set(kinds)) > 1 or kinds[0] not in _PAIRS else ():
+        gtypes = list(map(_DTYPE, given))
+        kinds = list(zip(ptypes, gtypes))
+        one = len(set(kinds)) == 1
+        for k, (pt, gt) in zip(live, kinds) if not one or kinds[0] not in _PAIRS else ():
             if (pt, gt) not in _PAIRS:
                 raise TypeError(f"AdamW.step: gradient {k} is {gt} for a tensor of {pt}")
+        if list(map(_BYTES, moved)) != [n * _SIZE[t] for n, t in zip(sizes, ptypes)] or list(map(_BYTES, given)) != [n * _SIZE[t] for n, t in zip(sizes, gtypes)] \
+                or not all(map(_CONTIGUOUS, moved)):
+            raise ValueError("AdamW.step: a tensor has changed its shape, type or strides")
         table = self._table if moved is params else self._table[live]
-        table["p"], table["g"] = list(map(_POINTER, moved)), list(map(_POINTER, given))
+        table["p"], table["g"] = array.array("Q", map(_POINTER, moved)), array.array("Q", map(_POINTER, given))
         if len(lr) == 1:
             table["lr"], table["weight_decay"] = lr[0], decay[0]
         else:
             table["lr"], table["weight_decay"] = [lr[self._group_of[k]] for k in live], [decay[self._group_of[k]] for k in live]
-        buckets = [(kinds[0], table)] if kinds.count(kinds[0]) == len(kinds) else \
-            [(kind, np.ascontiguousarray(table[[i for i, other in enumerate(kinds) if other == kind]])) for kind in dict.fromkeys(kinds)]
+        buckets = [(kinds[0], table)] if one else [(kind, np.ascontiguousarray(table[[i for i, other in enumerate(kinds) if other == kind]])) for kind in dict.fromkeys(kinds)]
+        m8, v8 = (None, None) if self.state_bits == 32 else (self.exp_avg_exponent.data_ptr(), self.exp_avg_sq_exponent.data_ptr())
         for n, ((pt, gt), part) in enumerate(buckets):
-            _ADAMW_STEP(device, part.ctypes.data, len(part), _TYPES[pt], _TYPES[gt], self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                        _lib.ptr(self.exp_avg_exponent), _lib.ptr(self.exp_avg_sq_exponent), self.betas[0], self.betas[1], self.eps, scale,
-                        self._state.data_ptr(), 1 if n + 1 == len(buckets) else 0)
+            _ADAMW_STEP(device, part.ctypes.data, len(part), _TYPES[pt], _TYPES[gt], self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), m8, v8,
+                        self.betas[0], self.betas[1], self.eps, scale, self._state.data_ptr(), 1 if n + 1 == len(buckets) else 0)
         torch.autograd.graph.increment_version(moved if not self._inference else [p for p in moved if not p.is_inference()])
 
     def zero_grad(self, set_to_none: bool = True) -> None:
