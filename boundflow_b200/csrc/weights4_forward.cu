@@ -4,8 +4,8 @@
 namespace bf {
 namespace {
 
-constexpr int X_BYTES = 40 * 1024;   // parts of the rows: with the ring, two blocks share an SM
-constexpr int X_MOST = 150 * 1024;   // and what a block alone on an SM has left of its 227 KB
+constexpr int SHARED_OF_TWO = 112 * 1024;  // shared memory of a block where two share an SM
+constexpr int X_MOST = 120 * 1024;   // and what a block alone on an SM has left of its 227 KB beside the ring and 32 KB of sums
 
 __device__ __forceinline__ void centre_radius(float a, float b, int mode, int relu_in, float& c, float& r) {
   if (mode == BF_IN_LOWER_UPPER) {
@@ -19,112 +19,145 @@ __device__ __forceinline__ void centre_radius(float a, float b, int mode, int re
   }
 }
 
-__device__ __forceinline__ void load8(const float* p, int left, bool wide, float (&v)[8]) {
-  if (wide && left >= 8) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
+// Eight neighbours of a row, as they lie in memory.
+template <int P> struct Eight { uint4 q; };
+template <> struct Eight<3> { uint4 q, r; };
+template <int P>
+__device__ __forceinline__ Eight<P> load8(const void* base, long long at, int left, bool wide) {
+  Eight<P> e;
+  if (P == 3) {
+    const float* p = static_cast<const float*>(base) + at;
+    if (wide && left >= 8) return *reinterpret_cast<const Eight<P>*>(p);
+    float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
-  }
-}
-// Eight 16-bit numbers as four words.
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int left, bool wide) {
-  if (wide && left >= 8) return *reinterpret_cast<const uint4*>(p);
-  uint32_t v[4];
+    memcpy(&e, v, sizeof e);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (wide && left >= 8) return *reinterpret_cast<const Eight<P>*>(p);
+    uint16_t v[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = (2 * j < left ? p[2 * j] : 0) | ((uint32_t)(2 * j + 1 < left ? p[2 * j + 1] : 0) << 16);
-  return make_uint4(v[0], v[1], v[2], v[3]);
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0;
+    memcpy(&e, v, sizeof e);
+  }
+  return e;
 }
 __device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // Parts of the rows' columns [from, to) * 128 in shared memory: [step of 32 columns][product][part, tile][column][4 lanes][8 columns of the step], the 8 in the
-// order 0 4 1 5 2 6 3 7 that `weights_of` gives the codes of a word in.  Eight columns of a row are a thread's turn.
-template <int P, int NT, bool DUAL>
-__device__ __forceinline__ void stage_rows(const W4LinearArgs& p, int packed, int from, int to, int m0, int M, int cv, int step_bytes, int set_bytes, uint32_t xs) {
-  constexpr int SETS = DUAL ? 2 : 1;
-  const int blocks = (to - from) * (CHUNK / 8), n_in = p.w.n_in;
-  const int per = P == 3 ? 4 : 8;  // elements of a 16-byte piece
-  const bool wide = n_in % per == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0;
-  int m = 0, blk = threadIdx.x;
-  while (blk >= blocks) { blk -= blocks; ++m; }
-  while (m < M) {
-    const int k = from * CHUNK + blk * 8, left = n_in - k;
-    const long long at = (long long)(m0 + m) * n_in + k;
-    uint32_t o[SETS][P][4];
-    if (P == 1) {
-      const uint4 v = load8(static_cast<const uint16_t*>(p.a) + at, left, wide);
-      o[0][0][0] = __byte_perm(v.x, v.z, 0x5410);
-      o[0][0][1] = __byte_perm(v.x, v.z, 0x7632);
-      o[0][0][2] = __byte_perm(v.y, v.w, 0x5410);
-      o[0][0][3] = __byte_perm(v.y, v.w, 0x7632);
-    } else {
-      float v[SETS][8];
-      if (P == 2) {
-        const uint4 q = load8(static_cast<const uint16_t*>(p.a) + at, left, wide);
-        const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q4[j]));
-          v[0][2 * j] = f.x;
-          v[0][2 * j + 1] = f.y;
-        }
-      } else {
-        load8(static_cast<const float*>(p.a) + at, left, wide, v[0]);
-        if (DUAL) {
-          load8(p.b + at, left, wide, v[SETS - 1]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) centre_radius(v[0][j], v[SETS - 1][j], p.mode, p.relu_in, v[0][j], v[SETS - 1][j]);
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < SETS; ++s)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t q[P];
-          two_numbers_checked<P>(v[s][j], v[s][j + 4], q);
-#pragma unroll
-          for (int i = 0; i < P; ++i) o[s][i][j] = q[i];
-        }
-    }
-    const uint32_t dst = xs + (blk >> 2) * step_bytes + (blk & 3) * 16;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int j = packed ? m * P + i : i * NT * 8 + m;  // column, counted through the tiles
-      const uint32_t to_q = dst + ((j >> 3) * cv + (j & 7)) * 64;
-#pragma unroll
-      for (int s = 0; s < SETS; ++s) put16(to_q + s * set_bytes, o[s][i][0], o[s][i][1], o[s][i][2], o[s][i][3]);
-    }
-    blk += THREADS;
-    while (blk >= blocks) { blk -= blocks; ++m; }
-  }
-}
+// order 0 4 1 5 2 6 3 7 that `weights_of` gives the codes of a word in.  Eight columns of a row are a thread's turn, AHEAD of them are on their way at a time.
+template <int P, bool PACKED, int NT, bool DUAL>
+struct Stager {
+  static constexpr int SETS = DUAL ? 2 : 1, AHEAD = P == 1 ? 4 : DUAL ? 1 : 2;
+  Eight<P> raw[AHEAD][SETS];
+  int rows[AHEAD], pieces[AHEAD];
+  int item, items, piece, row, per_row;
 
-// PARTS instructions for NT tiles of 8 columns; DUAL: W c and |W| r; F: steps of 32 columns that share a scale (1, 2, or 4 and more).
-template <int PARTS, int NT, bool DUAL, int F>
-__global__ void __launch_bounds__(THREADS, PARTS * NT * (DUAL ? 2 : 1) > 6 ? 1 : 2) w4_forward_kernel(const W4LinearArgs p, const Split sp) {
+  __device__ __forceinline__ void begin(int from, int to, int M) {
+    per_row = (to - from) * (CHUNK / 8);
+    items = per_row * M;
+    item = piece = threadIdx.x;
+    row = 0;
+  }
+  __device__ __forceinline__ void fetch(const W4LinearArgs& p, int from, int m0, bool wide) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      rows[i] = -1;
+      if (item < items) {
+        while (piece >= per_row) { piece -= per_row; ++row; }
+        const int k = from * CHUNK + piece * 8;
+        const long long at = (long long)(m0 + row) * p.w.n_in + k;
+        raw[i][0] = load8<P>(p.a, at, p.w.n_in - k, wide);
+        if (DUAL) raw[i][SETS - 1] = load8<P>(p.b, at, p.w.n_in - k, wide);
+        rows[i] = row;
+        pieces[i] = piece;
+      }
+      item += blockDim.x;
+      piece += blockDim.x;
+    }
+  }
+  __device__ __forceinline__ void put(const W4LinearArgs& p, int cv, int step_bytes, int set_bytes, uint32_t xs) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (rows[i] < 0) break;
+      uint32_t o[SETS][P][4];
+      if (P == 1) {
+        const uint4 v = raw[i][0].q;
+        o[0][0][0] = __byte_perm(v.x, v.z, 0x5410);
+        o[0][0][1] = __byte_perm(v.x, v.z, 0x7632);
+        o[0][0][2] = __byte_perm(v.y, v.w, 0x5410);
+        o[0][0][3] = __byte_perm(v.y, v.w, 0x7632);
+      } else {
+        float v[SETS][8];
+        if (P == 2) {
+          const uint32_t q4[4] = {raw[i][0].q.x, raw[i][0].q.y, raw[i][0].q.z, raw[i][0].q.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q4[j]));
+            v[0][2 * j] = f.x;
+            v[0][2 * j + 1] = f.y;
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < SETS; ++s) memcpy(v[s], &raw[i][s], 32);
+          if (DUAL) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) centre_radius(v[0][j], v[SETS - 1][j], p.mode, p.relu_in, v[0][j], v[SETS - 1][j]);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < SETS; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t q[P];
+            two_numbers_checked<P>(v[s][j], v[s][j + 4], q);
+#pragma unroll
+            for (int n = 0; n < P; ++n) o[s][n][j] = q[n];
+          }
+      }
+      const uint32_t dst = xs + (pieces[i] >> 2) * step_bytes + (pieces[i] & 3) * 16;
+#pragma unroll
+      for (int n = 0; n < P; ++n) {
+        const int j = PACKED ? rows[i] * P + n : n * NT * 8 + rows[i];  // column, counted through the tiles
+        const uint32_t to = dst + ((j >> 3) * cv + (j & 7)) * 64;
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) put16(to + s * set_bytes, o[s][n][0], o[s][n][1], o[s][n][2], o[s][n][3]);
+      }
+    }
+  }
+};
+
+// P parts of a row, side by side in the columns of NT tiles (PACKED) or an instruction each for NT tiles of 8 rows; DUAL: W c and |W| r; F: steps of 32 columns
+// that share a scale (1, 2, or 4 and more).
+template <int P, bool PACKED, int NT, bool DUAL, int F>
+__global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1) > 6 ? 1 : 2) w4_forward_kernel(const W4LinearArgs p, const Split sp) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int Q = PARTS * NT, SETS = DUAL ? 2 : 1;
+  constexpr int Q = (PACKED ? 1 : P) * NT, SETS = DUAL ? 2 : 1, COUNT = PACKED ? P : 1;
   const W4 w = p.w;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int kw = warp % sp.kw, rw = warp / sp.kw, rows_cta = TILE_N * (WARPS / sp.kw);
-  const int rank = blockIdx.x % sp.cluster;
-  const int nb = (blockIdx.x / sp.cluster) * rows_cta, n0 = nb + rw * TILE_N;
+  const int kw = warp & (sp.kw - 1), rw = warp >> sp.kw_log2;
+  const int rank = blockIdx.x & (sp.cluster - 1);
+  const int n0 = ((blockIdx.x >> sp.cluster_log2) * sp.rw + rw) * TILE_N;
   const int m0 = blockIdx.y * sp.tile_m, M = min(sp.tile_m, p.M - m0);
-  const int parts = p.type == BF_TYPE_F32 ? 3 : p.type == BF_TYPE_F16 ? 2 : 1;
-  const int cv = NT > 1 ? 8 : sp.packed ? M * parts : M;  // columns of a tile that are held
-  const int chunks = (w.n_in + CHUNK - 1) / CHUNK, share = (chunks + sp.cluster - 1) / sp.cluster;
+  const int cv = NT > 1 ? 8 : M * COUNT;  // columns of a tile that are held
+  const int chunks = (w.n_in + CHUNK - 1) / CHUNK, share = (chunks + sp.cluster - 1) >> sp.cluster_log2;
   const int first = min(rank * share, chunks), end = min(first + share, chunks);
+  const int warps = sp.kw * sp.rw;
+  const uint32_t inbox = smem_of(smem), ring = inbox + sp.inbox + warp * (STAGES * STAGE_BYTES), xs = inbox + sp.inbox + warps * (STAGES * STAGE_BYTES);
+  const int set_bytes = Q * cv * 64, step_bytes = SETS * set_bytes;
+  const bool wide = w.n_in % (P == 3 ? 4 : 8) == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0;
+  Stager<P, PACKED, NT, DUAL> stager;
+  int to = min(first + sp.per_phase, end);
+  stager.begin(first, to, M);
+  stager.fetch(p, first, m0, wide);  // before the codes: behind a ring of them in every warp these would wait for the memory's first microsecond
+  if (sp.cluster > 1) cluster_arrive();  // (before the sums go out all blocks of the cluster have to be there)
+
   const int groups = w.groups();
   const int pitch = (int)w.pitch();
-  const uint32_t ring = smem_of(smem) + warp * (STAGES * STAGE_BYTES), xs = smem_of(smem) + RING_BYTES;
-  const int set_bytes = Q * cv * 64, step_bytes = SETS * set_bytes;
   const int rows = max(0, min(TILE_N, w.n_out - n0));
   const uint8_t* codes = w.codes + (lane >> 2 < rows ? (long long)(n0 + (lane >> 2)) * pitch + (lane & 3) * 16 : 0);
-
   float tot[SETS][2][NT][4];
 #pragma unroll
   for (int s = 0; s < SETS; ++s)
@@ -136,10 +169,10 @@ __global__ void __launch_bounds__(THREADS, PARTS * NT * (DUAL ? 2 : 1) > 6 ? 1 :
         for (int i = 0; i < 4; ++i) tot[s][r][j][i] = 0.f;
 
   int next = first + kw;  // the chunk that is copied next
-  auto load_next = [&](uint32_t to) {
+  auto load_next = [&](uint32_t at) {
     if (next < end) {
-      load_codes(to, codes + next * (CHUNK / 2), 8LL * pitch, rows, pitch - next * (CHUNK / 2), lane);
-      load_scales(to, w, groups, n0, next, lane);
+      load_codes(at, codes + next * (CHUNK / 2), 8LL * pitch, rows, pitch - next * (CHUNK / 2), lane);
+      load_scales(at, w, groups, n0, next, lane);
     }
     copies_begin();
     next += sp.kw;
@@ -147,12 +180,17 @@ __global__ void __launch_bounds__(THREADS, PARTS * NT * (DUAL ? 2 : 1) > 6 ? 1 :
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load_next(ring + s * STAGE_BYTES);
   int slot = 0;
-  for (int from = first; from < end; from += sp.per_phase) {
-    const int to = min(from + sp.per_phase, end);
-    if (from != first) __syncthreads();
-    if (parts == 3) stage_rows<3, NT, DUAL>(p, sp.packed, from, to, m0, M, cv, step_bytes, set_bytes, xs);
-    if (!DUAL && parts == 2) stage_rows<2, NT, false>(p, sp.packed, from, to, m0, M, cv, step_bytes, set_bytes, xs);
-    if (!DUAL && parts == 1) stage_rows<1, NT, false>(p, sp.packed, from, to, m0, M, cv, step_bytes, set_bytes, xs);
+  for (int from = first; from < end; from = to, to = min(from + sp.per_phase, end)) {
+    if (from != first) {
+      __syncthreads();
+      stager.begin(from, to, M);
+      stager.fetch(p, from, m0, wide);
+    }
+    while (true) {
+      stager.put(p, cv, step_bytes, set_bytes, xs);
+      if (stager.item - threadIdx.x >= stager.items) break;
+      stager.fetch(p, from, m0, wide);
+    }
     __syncthreads();
     for (int c = from + kw; c < to; c += sp.kw) {
       copies_wait<STAGES - 2>();
@@ -221,41 +259,56 @@ __global__ void __launch_bounds__(THREADS, PARTS * NT * (DUAL ? 2 : 1) > 6 ? 1 :
       }
     }
   }
-  // Sums over the warps that split the columns, then over the blocks that did, each in order.
-  constexpr int CC = SETS * NT * 8;
-  float* red = reinterpret_cast<float*>(smem);  // [kw][CC][rows of the block and a pad]
-  const int line = rows_cta + 4;
+  // A warp puts its sums beside its ring, a row to a lane, adds a row's parts, and sends them to the block of the cluster that finishes the row (each takes as many
+  // rows of every tile): [product, row of the inputs][warp of the columns][row].  The sums over the columns are taken there, in a fixed order.
+  const int sources = sp.cluster * sp.kw, each_log2 = 5 - sp.cluster_log2, mine = sp.rw << each_log2;
   copies_wait<0>();
-  __syncthreads();
+  __syncwarp();
 #pragma unroll
   for (int s = 0; s < SETS; ++s)
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          red[(kw * CC + (s * NT + j) * 8 + 2 * t + (i & 1)) * line + rw * TILE_N + r * 16 + g + (i >> 1) * 8] = tot[s][r][j][i];
-  __syncthreads();
-  const int count = sp.packed ? parts : 1;
-  float* own = red + sp.kw * CC * line;  // [product][row of the tile][rows of the block]
-  for (int i = threadIdx.x; i < SETS * M * rows_cta; i += THREADS) {
-    const int row = i % rows_cta, j = i / rows_cta, s = DUAL && j >= M ? 1 : 0, m = j - s * M;
-    const float* at = red + (s * NT * 8 + m * count) * line + row;
-    float v = 0.f;
-    for (int k = 0; k < sp.kw; ++k)
-      for (int part = 0; part < count; ++part) v += at[(k * CC + part) * line];
-    own[i] = v;
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (((s * NT + j) * 8 + 2 * t + (i & 1)) * 36 + r * 16 + g + (i >> 1) * 8) * 4), "f"(tot[s][r][j][i]) : "memory");
+  __syncwarp();
+  if (sp.cluster > 1) cluster_wait();
+  {
+    const int owner = lane >> each_log2;
+    uint32_t at = inbox + ((rank * sp.kw + kw) * mine + (rw << each_log2) + lane - (owner << each_log2)) * 4;
+    if (sp.cluster > 1) at = cluster_address(at, owner);
+#pragma unroll
+    for (int s = 0; s < SETS; ++s)
+      for (int m = 0; m < M; ++m) {
+        const uint32_t from = ring + ((s * NT * 8 + m * COUNT) * 36 + lane) * 4;
+        float v = __uint_as_float(lds32(from));
+#pragma unroll
+        for (int n = 1; n < COUNT; ++n) v += __uint_as_float(lds32(from + n * 36 * 4));
+        cluster_store(at + (s * M + m) * sources * mine * 4, v, sp.cluster > 1);
+      }
   }
   if (sp.cluster > 1) cluster_barrier();
   else __syncthreads();
-  const int mine = rows_cta / sp.cluster;  // rows of the block that this one finishes
-  for (int i = threadIdx.x; i < mine * M; i += THREADS) {
-    const int m = i / mine, row = rank * mine + i - m * mine, n = nb + row;
+  const float* box = reinterpret_cast<const float*>(smem);
+  for (int i = threadIdx.x; i < mine * M; i += blockDim.x) {
+    const int m = __umulhi(i, sp.mine_inverse), row = i - m * mine;  // i / mine
+    const int tile = row >> each_log2, n = ((blockIdx.x >> sp.cluster_log2) * sp.rw + tile) * TILE_N + (rank << each_log2) + row - (tile << each_log2);
     if (n >= w.n_out) continue;
     float sum[2];
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) sum[s] = cluster_sum(own + (s * M + m) * rows_cta + row, sp.cluster);
+    for (int s = 0; s < SETS; ++s) {
+      const float* at = box + (s * M + m) * sources * mine + row;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      int k = 0;
+      for (; k + 4 <= sources; k += 4, at += 4 * mine) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] += at[x * mine];
+      }
+      for (; k < sources; ++k, at += mine) v[0] += *at;
+      sum[s] = (v[0] + v[1]) + (v[2] + v[3]);
+    }
     const float c = sum[0] + (p.bias ? load_any(p.bias, p.bias_type, n) : 0.f);
     const long long at = (long long)(m0 + m) * w.n_out + n;
     if (DUAL) {
@@ -265,16 +318,15 @@ __global__ void __launch_bounds__(THREADS, PARTS * NT * (DUAL ? 2 : 1) > 6 ? 1 :
       store_any(p.y, p.type, at, c);
     }
   }
-  if (sp.cluster > 1) cluster_barrier();  // the others may still read this block's sums
 }
 
-template <int PARTS, int NT, bool DUAL>
+template <int P, bool PACKED, int NT, bool DUAL>
 int forward(const W4LinearArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
   static SmemOptIn table[3];
+  constexpr int Q = (PACKED ? 1 : P) * NT, SETS = DUAL ? 2 : 1, COUNT = PACKED ? P : 1;
   const int tiles_n = ceil_div(p.w.n_out, TILE_N), chunks = ceil_div(p.w.n_in, CHUNK);
-  const int parts = p.type == BF_TYPE_F32 ? 3 : p.type == BF_TYPE_F16 ? 2 : 1;
-  const int cv = NT > 1 ? 8 : sp.packed ? sp.tile_m * parts : sp.tile_m;
-  const int chunk_bytes = 4 * (DUAL ? 2 : 1) * PARTS * NT * cv * 64;
+  const int cv = NT > 1 ? 8 : sp.tile_m * COUNT;
+  const int chunk_bytes = 4 * SETS * Q * cv * 64;
   // 16 warps an SM: the columns are split as often as that takes.  Over a cluster while a block's part of the rows is long (every block makes
   // parts of what it reads, 4096 elements take about a microsecond), else over the warps of a block.
   const long long units = (long long)tiles_n * tiles_m;
@@ -285,14 +337,22 @@ int forward(const W4LinearArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
   sp.kw = std::min(WARPS, split / sp.cluster);
   while (sp.kw * chunk_bytes > X_MOST) sp.kw /= 2;  // the warps of a block take a chunk each
   sp.cluster = std::min(8, std::max(sp.cluster, split / sp.kw));
+  sp.kw_log2 = log2_of(sp.kw);
+  sp.cluster_log2 = log2_of(sp.cluster);
+  sp.rw = WARPS / sp.kw;
+  const int mine = sp.rw * TILE_N / sp.cluster;
+  sp.mine_inverse = mine == 1 ? 0xffffffffu : (unsigned)((0x100000000ULL + mine - 1) / mine);
   const int share = ceil_div(chunks, sp.cluster);
-  sp.per_phase = std::max(sp.kw, X_BYTES / chunk_bytes / sp.kw * sp.kw);
-  const int x_bytes = std::min(sp.per_phase, share) * chunk_bytes;
-  const long long blocks = (long long)ceil_div(p.w.n_out, TILE_N * (WARPS / sp.kw)) * sp.cluster;
-  const int smem = RING_BYTES + x_bytes;
-  if (p.w.group_log2 == 5) return launch_clustered(w4_forward_kernel<PARTS, NT, DUAL, 1>, "w4_forward_kernel", table[0], p, sp, blocks, tiles_m, smem, stream);
-  if (p.w.group_log2 == 6) return launch_clustered(w4_forward_kernel<PARTS, NT, DUAL, 2>, "w4_forward_kernel", table[1], p, sp, blocks, tiles_m, smem, stream);
-  return launch_clustered(w4_forward_kernel<PARTS, NT, DUAL, 4>, "w4_forward_kernel", table[2], p, sp, blocks, tiles_m, smem, stream);
+  sp.inbox = ceil_div((long long)sp.kw * SETS * sp.tile_m * TILE_N * sp.rw * 4, 128) * 128;
+  const int room = SHARED_OF_TWO - sp.inbox - RING_BYTES;  // for the parts of the rows, with two blocks on an SM
+  sp.per_phase = std::max(sp.kw, room / chunk_bytes / sp.kw * sp.kw);
+  const int smem = sp.inbox + RING_BYTES + std::min(sp.per_phase, share) * chunk_bytes;
+  const long long blocks = (long long)ceil_div(tiles_n, sp.rw) * sp.cluster;
+  if (p.w.group_log2 == 5)
+    return launch_clustered(w4_forward_kernel<P, PACKED, NT, DUAL, 1>, "w4_forward_kernel", table[0], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  if (p.w.group_log2 == 6)
+    return launch_clustered(w4_forward_kernel<P, PACKED, NT, DUAL, 2>, "w4_forward_kernel", table[1], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  return launch_clustered(w4_forward_kernel<P, PACKED, NT, DUAL, 4>, "w4_forward_kernel", table[2], p, sp, blocks, tiles_m, THREADS, smem, stream);
 }
 
 }  // namespace
@@ -302,8 +362,9 @@ int launch_w4_linear(const W4LinearArgs& all, cudaStream_t stream) {
   const bool dual = all.b != nullptr;
   const int parts = all.type == BF_TYPE_F32 ? 3 : all.type == BF_TYPE_F16 ? 2 : 1;
   const int side = all.M * parts;  // columns that the rows' parts fill side by side: fewer instructions up to two tiles
-  sp.packed = side <= 8 || (side <= 16 && parts > 1);
-  const int nt = sp.packed ? (side <= 8 ? 1 : 2) : all.M <= 8 ? 1 : 2;
+  // (9 and 10 rows in three parts: 4 tiles side by side, 6 otherwise)
+  sp.packed = side <= 8 || (side <= 16 && parts > 1) || (side > 24 && side <= 32 && parts == 3 && !dual);
+  const int nt = sp.packed ? (side <= 8 ? 1 : side <= 16 ? 2 : 4) : all.M <= 8 ? 1 : 2;
   sp.tile_m = sp.packed ? all.M : std::min(all.M, 8 * nt);
   const long long tiles = ceil_div(all.M, sp.tile_m);
   for (long long first = 0; first < tiles; first += MOST_TILES) {
@@ -317,11 +378,15 @@ int launch_w4_linear(const W4LinearArgs& all, cudaStream_t stream) {
     p.y2 = dual ? all.y2 + skip * all.w.n_out : nullptr;
     int rc;
     if (dual)
-      rc = sp.packed ? (nt == 1 ? forward<1, 1, true>(p, sp, here, stream) : forward<1, 2, true>(p, sp, here, stream))
-                     : nt == 1 ? forward<3, 1, true>(p, sp, here, stream) : forward<3, 2, true>(p, sp, here, stream);
-    else if (sp.packed || parts == 1) rc = nt == 1 ? forward<1, 1, false>(p, sp, here, stream) : forward<1, 2, false>(p, sp, here, stream);
-    else if (parts == 2) rc = forward<2, 2, false>(p, sp, here, stream);
-    else rc = nt == 1 ? forward<3, 1, false>(p, sp, here, stream) : forward<3, 2, false>(p, sp, here, stream);
+      rc = sp.packed ? (nt == 1 ? forward<3, true, 1, true>(p, sp, here, stream) : forward<3, true, 2, true>(p, sp, here, stream))
+                     : (nt == 1 ? forward<3, false, 1, true>(p, sp, here, stream) : forward<3, false, 2, true>(p, sp, here, stream));
+    else if (parts == 3)
+      rc = sp.packed ? (nt == 1 ? forward<3, true, 1, false>(p, sp, here, stream) : nt == 2 ? forward<3, true, 2, false>(p, sp, here, stream)
+                                                                                            : forward<3, true, 4, false>(p, sp, here, stream))
+                     : (nt == 1 ? forward<3, false, 1, false>(p, sp, here, stream) : forward<3, false, 2, false>(p, sp, here, stream));
+    else if (parts == 2)
+      rc = !sp.packed ? forward<2, false, 2, false>(p, sp, here, stream) : nt == 1 ? forward<2, true, 1, false>(p, sp, here, stream) : forward<2, true, 2, false>(p, sp, here, stream);
+    else rc = nt == 1 ? forward<1, true, 1, false>(p, sp, here, stream) : forward<1, false, 2, false>(p, sp, here, stream);
     if (rc != BF_OK) return rc;
   }
   return BF_OK;

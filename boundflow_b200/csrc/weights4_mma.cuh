@@ -104,10 +104,14 @@ __device__ __forceinline__ void two_numbers_checked(float a, float b, uint32_t (
 // How the work is split over blocks.
 struct Split {
   int packed;     // parts of a row side by side in the instruction's columns
-  int kw;         // forward: warps of a block that share rows and split columns (8 / kw row tiles a block)
+  int kw;         // forward: warps of a block that share rows and split columns
+  int rw;         // forward: row tiles of a block (kw * rw warps)
   int cluster;    // blocks that split the columns (forward) or the outputs (rows)
+  int kw_log2, cluster_log2;
   int per_phase;  // forward: chunks whose parts are in shared memory at a time
   int tile_m;     // rows of a block
+  int inbox;      // forward: bytes of the sums that come from the warps that split the columns
+  unsigned mine_inverse;  // forward: 2^32 over the rows that a block finishes
 };
 
 // Lanes copy a stage: codes [32 rows][64 bytes], scales of the chunk's groups.  `codes` is the lane's first 16 bytes (row lane / 4, piece lane % 4),
@@ -153,18 +157,29 @@ __device__ __forceinline__ float cluster_sum(const float* p, int blocks) {
     if (k < blocks) s += v[k];
   return s;
 }
+__device__ __forceinline__ uint32_t cluster_address(uint32_t at, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_store(uint32_t at, float v, bool cluster) {
+  if (cluster) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+  else asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <typename Args>
-int launch_clustered(void (*kernel)(Args, Split), const char* name, SmemOptIn& table, const Args& p, const Split& sp, long long blocks, int tiles_m, int smem,
-                     cudaStream_t stream) {
+int launch_clustered(void (*kernel)(Args, Split), const char* name, SmemOptIn& table, const Args& p, const Split& sp, long long blocks, int tiles_m, int threads,
+                     int smem, cudaStream_t stream) {
   const int rc = ensure_dynamic_smem(kernel, smem, table, name);
   if (rc != BF_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, tiles_m);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -178,6 +193,11 @@ int launch_clustered(void (*kernel)(Args, Split), const char* name, SmemOptIn& t
   return BF_OK;
 }
 
+int log2_of(int v) {
+  int l = 0;
+  while ((1 << l) < v) ++l;
+  return l;
+}
 int power_below(int v) {
   int p = 1;
   while (2 * p <= v) p *= 2;

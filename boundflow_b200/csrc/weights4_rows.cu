@@ -234,9 +234,9 @@ int backward(const W4RowsArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
   const int rows_bytes = WARPS * (DUAL ? 2 : 1) * (PACKED ? 1 : P * NT) * cv * 64;
   const int smem = RING_BYTES + rows_bytes;  // (the sums at the end need less)
   const long long blocks = (long long)kblocks * sp.cluster;
-  if (p.w.group_log2 == 5) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 1>, "w4_rows_kernel", table[0], p, sp, blocks, tiles_m, smem, stream);
-  if (p.w.group_log2 == 6) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 2>, "w4_rows_kernel", table[1], p, sp, blocks, tiles_m, smem, stream);
-  return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 4>, "w4_rows_kernel", table[2], p, sp, blocks, tiles_m, smem, stream);
+  if (p.w.group_log2 == 5) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 1>, "w4_rows_kernel", table[0], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  if (p.w.group_log2 == 6) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 2>, "w4_rows_kernel", table[1], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 4>, "w4_rows_kernel", table[2], p, sp, blocks, tiles_m, THREADS, smem, stream);
 }
 
 }  // namespace
