@@ -120,8 +120,8 @@ struct Stager {
       const uint32_t dst = xs + (pieces[i] >> 2) * step_bytes + (pieces[i] & 3) * 16;
 #pragma unroll
       for (int n = 0; n < P; ++n) {
-        const int j = PACKED ? rows[i] * P + n : n * NT * 8 + rows[i];  // column, counted through the tiles
-        const uint32_t to = dst + ((j >> 3) * cv + (j & 7)) * 64;
+        const int j = PACKED ? rows[i] * P + n : n * NT * cv + rows[i];  // column, counted through the tiles
+        const uint32_t to = dst + j * 64;
 #pragma unroll
         for (int s = 0; s < SETS; ++s) put16(to + s * set_bytes, o[s][n][0], o[s][n][1], o[s][n][2], o[s][n][3]);
       }

@@ -138,25 +138,6 @@ __device__ __forceinline__ uint32_t lds32(uint32_t at) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
-__device__ __forceinline__ float cluster_read(const float* p, uint32_t rank) {
-  uint32_t at;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_of(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-// The sum over the blocks of a cluster of what each has at `p`, in order; all of it is on its way before the first is added.
-__device__ __forceinline__ float cluster_sum(const float* p, int blocks) {
-  if (blocks == 1) return *p;
-  float v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < blocks ? cluster_read(p, k) : 0.f;
-  float s = v[0];
-#pragma unroll
-  for (int k = 1; k < 8; ++k)
-    if (k < blocks) s += v[k];
-  return s;
-}
 __device__ __forceinline__ uint32_t cluster_address(uint32_t at, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));

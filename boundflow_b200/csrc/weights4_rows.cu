@@ -16,14 +16,15 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
   constexpr int TURNS = (MT + 1) / 2;           // rows of a half warp
   const W4 w = p.w;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % sp.cluster, kb = blockIdx.x / sp.cluster;
+  const int rank = blockIdx.x & (sp.cluster - 1), kb = blockIdx.x >> sp.cluster_log2;  // (cluster is a power of two)
   const int m0 = blockIdx.y * sp.tile_m, M = min(sp.tile_m, p.M - m0);
   const int cv = PACKED ? M * P : (NT == 1 ? M : 8);
-  const int tiles = (w.n_out + TILE_N - 1) / TILE_N, share = (tiles + sp.cluster - 1) / sp.cluster;
+  const int tiles = (w.n_out + TILE_N - 1) / TILE_N, share = (tiles + sp.cluster - 1) >> sp.cluster_log2;
   const int first = min(rank * share, tiles), end = min(first + share, tiles);
   const int groups = w.groups();
   const long long pitch = w.pitch();
-  const uint32_t ring = smem_of(smem) + warp * (STAGES * STAGE_BYTES);
+  const uint32_t inbox = smem_of(smem) + RING_BYTES + WARPS * (SETS * Q * cv * 64), ring = smem_of(smem) + warp * (STAGES * STAGE_BYTES);
+  if (sp.cluster > 1) cluster_arrive();  // (before the sums go out all blocks of the cluster have to be there)
   const int set_bytes = Q * cv * 64;
   const uint32_t as = smem_of(smem) + RING_BYTES + warp * (SETS * set_bytes);  // [set][part, tile][column][32 outputs, in the order the lanes read them]
   // a lane makes the parts of two neighbouring outputs of every other row
@@ -82,6 +83,8 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
     }
   };
 
+  float av[SETS][TURNS][2];
+  rows_at(first + warp, av);  // before the codes, which would keep these waiting for the memory's first microsecond
   int next = first + warp;
   auto load_next = [&](uint32_t to) {
     if (next < end) {
@@ -94,8 +97,6 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load_next(ring + s * STAGE_BYTES);
-  float av[SETS][TURNS][2];
-  rows_at(first + warp, av);
   int slot = 0;
   for (int tile = first + warp; tile < end; tile += WARPS) {
     float now[SETS][TURNS][2];
@@ -132,8 +133,8 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
               two_numbers_checked<P>(now[s][i][0] * (s == 0 ? f0 : fabsf(f0)), now[s][i][1] * (s == 0 ? f1 : fabsf(f1)), q);
 #pragma unroll
               for (int part = 0; part < P; ++part) {
-                const int j = PACKED ? m * P + part : part * NT * 8 + m;
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(place + s * set_bytes + ((j >> 3) * cv + (j & 7)) * 64), "r"(q[part]) : "memory");
+                const int j = PACKED ? m * P + part : part * NT * cv + m;  // column, counted through the tiles
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(place + s * set_bytes + j * 64), "r"(q[part]) : "memory");
               }
             }
           }
@@ -174,11 +175,16 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
       }
     }
   }
-  // Sums over the warps, eight columns of rows at a time, then over the blocks of the cluster, each in order.
-  float* red = reinterpret_cast<float*>(smem);  // [warp][8][128 and a pad]
+  // Sums over the warps, eight columns at a time, go to the block of the cluster that finishes the input features, [product, row][block][feature]; the sums over
+  // the blocks are taken there, each in a fixed order.
   constexpr int LINE = CHUNK + 4;
-  float* own = red + WARPS * 8 * LINE;          // [product][row][128]
+  float* red = reinterpret_cast<float*>(smem);  // [warp][8][128 and a pad]
+  const int each_log2 = 7 - sp.cluster_log2, mine = 1 << each_log2;
   copies_wait<0>();
+  if (sp.cluster > 1) cluster_wait();
+  const int feature = threadIdx.x & (CHUNK - 1), owner = feature >> each_log2;
+  uint32_t out = inbox + ((rank << each_log2) + feature - (owner << each_log2)) * 4;
+  if (sp.cluster > 1) out = cluster_address(out, owner);
 #pragma unroll
   for (int s = 0; s < SETS; ++s)
 #pragma unroll
@@ -193,25 +199,36 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
             red[(warp * 8 + 2 * t + (i & 1)) * LINE + r * 32 + 8 * (g & 3) + 4 * (g >> 2) + 2 * e + (i >> 1)] = acc[s][r][e][j][i];
       __syncthreads();
       const int here = PACKED ? M : min(8, M - j * 8);  // rows of the tile
-      for (int i = threadIdx.x; i < here * CHUNK; i += THREADS) {
-        const int m = i / CHUNK, k = i % CHUNK;
+      for (int m = threadIdx.x >> 7; m < here; m += THREADS / CHUNK) {
         float v = 0.f;
 #pragma unroll
         for (int q = 0; q < (PACKED ? P : 1); ++q)
 #pragma unroll
-          for (int x = 0; x < WARPS; ++x) v += red[(x * 8 + (PACKED ? m * P + q : m)) * LINE + k];
-        own[(s * M + j * 8 + m) * CHUNK + k] = v;
+          for (int x = 0; x < WARPS; ++x) v += red[(x * 8 + (PACKED ? m * P + q : m)) * LINE + feature];
+        cluster_store(out + (s * M + j * 8 + m) * CHUNK * 4, v, sp.cluster > 1);
       }
     }
   if (sp.cluster > 1) cluster_barrier();
   else __syncthreads();
-  const int mine = CHUNK / sp.cluster;
-  for (int i = threadIdx.x; i < mine * M; i += THREADS) {
-    const int m = i / mine, k = rank * mine + i - m * mine;
+  const float* box = reinterpret_cast<const float*>(smem + (inbox - smem_of(smem)));
+  for (int i = threadIdx.x; i < M << each_log2; i += THREADS) {
+    const int m = i >> each_log2, k = (rank << each_log2) + (i & (mine - 1));
     if (kb * CHUNK + k >= w.n_in) continue;
     float sum[2];
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) sum[s] = cluster_sum(own + (s * M + m) * CHUNK + k, sp.cluster);
+    for (int s = 0; s < SETS; ++s) {
+      const float* at = box + (s * M + m) * CHUNK + (i & (mine - 1));
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (sp.cluster < 4) {
+        for (int c = 0; c < sp.cluster; ++c) v[0] += at[c << each_log2];
+      } else {
+        for (int c = 0; c < sp.cluster; c += 4) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] += at[(c + x) << each_log2];
+        }
+      }
+      sum[s] = (v[0] + v[1]) + (v[2] + v[3]);
+    }
     const long long at = (long long)(m0 + m) * w.n_in + kb * CHUNK + k;
     if (DUAL) {
       static_cast<float*>(p.z)[at] = 0.5f * (sum[0] - sum[1]);
@@ -220,7 +237,6 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
       store_any(p.z, p.type, at, sum[0]);
     }
   }
-  if (sp.cluster > 1) cluster_barrier();
 }
 
 template <int P, bool PACKED, int NT, bool DUAL>
@@ -230,9 +246,10 @@ int backward(const W4RowsArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
   const long long units = (long long)kblocks * tiles_m;
   const int split = (int)std::max<long long>(1, std::min<long long>(ceil_div(tiles, WARPS), (2LL * SMS) / units));
   sp.cluster = std::min(8, power_below(split));
+  sp.cluster_log2 = log2_of(sp.cluster);
   const int cv = PACKED ? sp.tile_m * P : (NT == 1 ? sp.tile_m : 8);
   const int rows_bytes = WARPS * (DUAL ? 2 : 1) * (PACKED ? 1 : P * NT) * cv * 64;
-  const int smem = RING_BYTES + rows_bytes;  // (the sums at the end need less)
+  const int smem = RING_BYTES + rows_bytes + (DUAL ? 2 : 1) * sp.tile_m * CHUNK * 4;  // ring (the sums over the warps at the end need less), parts, sums of the cluster
   const long long blocks = (long long)kblocks * sp.cluster;
   if (p.w.group_log2 == 5) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 1>, "w4_rows_kernel", table[0], p, sp, blocks, tiles_m, THREADS, smem, stream);
   if (p.w.group_log2 == 6) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 2>, "w4_rows_kernel", table[1], p, sp, blocks, tiles_m, THREADS, smem, stream);
