@@ -47,43 +47,45 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[s][r][e][j][i] = 0.f;
 
-  auto rows_at = [&](int tile, float (&v)[SETS][TURNS][2]) {
+  // (as they lie in memory: a conversion here would wait for each load in turn)
+  constexpr int WORDS = P == 3 ? 2 : 1;
+  auto rows_at = [&](int tile, uint32_t (&v)[SETS][TURNS][WORDS]) {
     const int n = tile * TILE_N + 2 * pair;
+    const bool here = tile < end && n < w.n_out, two = n + 1 < w.n_out;
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
       const int m = 2 * i + odd;
 #pragma unroll
-      for (int s = 0; s < SETS; ++s) v[s][i][0] = v[s][i][1] = 0.f;
-      if (m < M && tile < end && n < w.n_out) {
-        const long long at = (long long)(m0 + m) * w.n_out + n;
-        const bool two = n + 1 < w.n_out;
-        if (P == 3) {
-#pragma unroll
-          for (int s = 0; s < SETS; ++s) {
-            const float* from = (s == 0 ? static_cast<const float*>(p.a) : p.b) + at;
+      for (int s = 0; s < SETS; ++s) {
+        v[s][i][0] = v[s][i][WORDS - 1] = 0;
+        if (m < M && here) {
+          const long long at = (long long)(m0 + m) * w.n_out + n;
+          if (P == 3) {
+            const uint32_t* from = reinterpret_cast<const uint32_t*>(s == 0 ? static_cast<const float*>(p.a) : p.b) + at;
             if (wide) {
-              const float2 f = *reinterpret_cast<const float2*>(from);
+              const uint2 f = *reinterpret_cast<const uint2*>(from);
               v[s][i][0] = f.x;
-              v[s][i][1] = f.y;
+              v[s][i][WORDS - 1] = f.y;
             } else {
               v[s][i][0] = from[0];
-              if (two) v[s][i][1] = from[1];
+              if (two) v[s][i][WORDS - 1] = from[1];
             }
+          } else {
+            const uint16_t* from = static_cast<const uint16_t*>(p.a) + at;
+            if (wide) v[0][i][0] = *reinterpret_cast<const uint32_t*>(from);
+            else v[0][i][0] = from[0] | (two ? (uint32_t)from[1] << 16 : 0u);
           }
-        } else {
-          uint32_t q;
-          const uint16_t* from = static_cast<const uint16_t*>(p.a) + at;
-          if (wide) q = *reinterpret_cast<const uint32_t*>(from);
-          else q = from[0] | (two ? (uint32_t)from[1] << 16 : 0u);
-          const float2 f = p.type == BF_TYPE_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q)) : __half22float2(*reinterpret_cast<const __half2*>(&q));
-          v[0][i][0] = f.x;
-          v[0][i][1] = f.y;
         }
       }
     }
   };
+  auto numbers = [&](const uint32_t (&v)[WORDS]) {
+    if (P == 3) return make_float2(__uint_as_float(v[0]), __uint_as_float(v[WORDS - 1]));
+    if (p.type == BF_TYPE_BF16) return make_float2(__uint_as_float(v[0] << 16), __uint_as_float(v[0] & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&v[0]));
+  };
 
-  float av[SETS][TURNS][2];
+  uint32_t av[SETS][TURNS][WORDS];
   rows_at(first + warp, av);  // before the codes, which would keep these waiting for the memory's first microsecond
   int next = first + warp;
   auto load_next = [&](uint32_t to) {
@@ -99,18 +101,16 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
   for (int s = 0; s < STAGES - 1; ++s) load_next(ring + s * STAGE_BYTES);
   int slot = 0;
   for (int tile = first + warp; tile < end; tile += WARPS) {
-    float now[SETS][TURNS][2];
+    float2 now[SETS][TURNS];
 #pragma unroll
-    for (int i = 0; i < TURNS; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (DUAL) {  // gradients of lower and upper bounds to those of centre and radius
-          now[0][i][j] = av[0][i][j] + av[SETS - 1][i][j];
-          now[SETS - 1][i][j] = av[SETS - 1][i][j] - av[0][i][j];
-        } else {
-          now[0][i][j] = av[0][i][j];
-        }
+    for (int i = 0; i < TURNS; ++i) {
+      now[0][i] = numbers(av[0][i]);
+      if (DUAL) {  // gradients of lower and upper bounds to those of centre and radius
+        const float2 lo = now[0][i], up = numbers(av[SETS - 1][i]);
+        now[0][i] = make_float2(lo.x + up.x, lo.y + up.y);
+        now[SETS - 1][i] = make_float2(up.x - lo.x, up.y - lo.y);
       }
+    }
     rows_at(tile + WARPS, av);
     copies_wait<STAGES - 2>();
     __syncwarp();
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
 #pragma unroll
             for (int s = 0; s < SETS; ++s) {
               uint32_t q[P];
-              two_numbers_checked<P>(now[s][i][0] * (s == 0 ? f0 : fabsf(f0)), now[s][i][1] * (s == 0 ? f1 : fabsf(f1)), q);
+              two_numbers_checked<P>(now[s][i].x * (s == 0 ? f0 : fabsf(f0)), now[s][i].y * (s == 0 ? f1 : fabsf(f1)), q);
 #pragma unroll
               for (int part = 0; part < P; ++part) {
                 const int j = PACKED ? m * P + part : part * NT * cv + m;  // column, counted through the tiles
