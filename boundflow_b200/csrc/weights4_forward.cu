@@ -20,7 +20,7 @@ __device__ __forceinline__ void centre_radius(float a, float b, int mode, int re
 }
 
 // Eight neighbours of a row, as they lie in memory.
-template <int P> struct Eight { uint4 q; };
+template <int P> struct Eight { uint4 q; };  // (16-bit numbers)
 template <> struct Eight<3> { uint4 q, r; };
 template <int P>
 __device__ __forceinline__ Eight<P> load8(const void* base, long long at, int left, bool wide) {
@@ -46,11 +46,17 @@ __device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint3
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Digits (P = DIGITS): up to four 16-bit rows as whole numbers of four 8-bit digits, counted in 2^(e - 156) with e the biased exponent of the largest of the row's
+// columns that share a scale (128 of them at most).  A bfloat16 number is held exactly down to 2^-22 of that largest, a half down to 2^-19, and what is smaller within 2^-31 of it.  The codes
+// turn into 8-bit numbers, 16 (code - 8), with three operations a word instead of eleven, the integer instruction takes twice as many columns, and its sums are
+// exact; a factor for each column brings them back.  Rows of infinities count those, times infinity; a NaN makes the factor one.
+constexpr int DIGITS = 4;
+
 // Parts of the rows' columns [from, to) * 128 in shared memory: [step of 32 columns][product][part, tile][column][4 lanes][8 columns of the step], the 8 in the
-// order 0 4 1 5 2 6 3 7 that `weights_of` gives the codes of a word in.  Eight columns of a row are a thread's turn, AHEAD of them are on their way at a time.
+// order 0 4 1 5 2 6 3 7 that `weights_of` gives the codes of a word in (digits: 0 2 4 6 1 3 5 7).  Eight columns of a row are a thread's turn, AHEAD of them are on their way at a time.
 template <int P, bool PACKED, int NT, bool DUAL>
 struct Stager {
-  static constexpr int SETS = DUAL ? 2 : 1, AHEAD = P == 1 ? 4 : DUAL ? 1 : 2;
+  static constexpr int SETS = DUAL ? 2 : 1, AHEAD = P == 1 || P == DIGITS ? 4 : DUAL ? 1 : 2;
   Eight<P> raw[AHEAD][SETS];
   int rows[AHEAD], pieces[AHEAD];
   int item, items, piece, row, per_row;
@@ -78,12 +84,67 @@ struct Stager {
       piece += blockDim.x;
     }
   }
-  __device__ __forceinline__ void put(const W4LinearArgs& p, int cv, int step_bytes, int set_bytes, uint32_t xs) {
+  // Digits of eight columns: their word holds the four, byte by byte (balanced, -128 to 127); a transposition of bytes gives each digit's word of four columns.
+  __device__ __forceinline__ void put_digits(const Eight<P>& e, int type, int lanes, int row, int piece, int step_bytes, uint32_t xs, uint32_t factors) {
+    const uint32_t q4[4] = {e.q.x, e.q.y, e.q.z, e.q.w};
+    float v[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = type == BF_TYPE_BF16 ? make_float2(__uint_as_float(q4[j] << 16), __uint_as_float(q4[j] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&q4[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+      top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+    const uint32_t half = 0xffffu << (threadIdx.x & 16);  // the 16 lanes of a chunk's columns; `lanes` of them share a scale
+    for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(half, top, o));
+    const int exponent = max((int)(top >> 23), 30);  // (below 2^-97 the digits' unit stays)
+    uint32_t z[8];
+    if (exponent < 255) {
+      const float scale = __uint_as_float((uint32_t)(283 - exponent) << 23);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = ((uint32_t)__float2int_rn(v[j] * scale) + 0x00808080u) ^ 0x00808080u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = isinf(v[j]) ? (v[j] > 0.f ? 0x00000001u : 0x000000ffu) : 0u;
+    }
+    const uint32_t to = xs + (piece >> 2) * step_bytes + (row * 4 * 4 + (piece & 3)) * 8;
+    uint32_t o[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t a = __byte_perm(z[h], z[h + 2], 0x5140), b = __byte_perm(z[h], z[h + 2], 0x7362);
+      const uint32_t c = __byte_perm(z[h + 4], z[h + 6], 0x5140), d = __byte_perm(z[h + 4], z[h + 6], 0x7362);
+      o[h][0] = __byte_perm(a, c, 0x5410);
+      o[h][1] = __byte_perm(a, c, 0x7632);
+      o[h][2] = __byte_perm(b, d, 0x5410);
+      o[h][3] = __byte_perm(b, d, 0x7632);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(to + d * 32), "r"(o[0][d]), "r"(o[1][d]) : "memory");
+    if ((piece & (lanes - 1)) == 0) {  // 2^(e - 156) / 16 and the digits' places
+      float f[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        f[d] = ldexpf(1.f, exponent - 160 + 8 * d);
+        if (exponent == 255) f[d] = top > 0x7f800000u ? __int_as_float(0x7fffffff) : d == 0 ? __int_as_float(0x7f800000) : 0.f;
+      }
+      asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(factors + (piece / lanes * NT * 8 + row * 4) * 4), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
+    }
+  }
+  __device__ __forceinline__ void put(const W4LinearArgs& p, int cv, int step_bytes, int set_bytes, uint32_t xs, uint32_t factors) {
+    if (P == DIGITS) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (rows[i] < 0) break;
+        put_digits(raw[i][0], p.type, 4 << min(p.w.group_log2 - 5, 2), rows[i], pieces[i], step_bytes, xs, factors);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (rows[i] < 0) break;
       uint32_t o[SETS][P][4];
-      if (P == 1) {
+      if (P == 1 || P == DIGITS) {
         const uint4 v = raw[i][0].q;
         o[0][0][0] = __byte_perm(v.x, v.z, 0x5410);
         o[0][0][1] = __byte_perm(v.x, v.z, 0x7632);
@@ -146,7 +207,8 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
   const int first = min(rank * share, chunks), end = min(first + share, chunks);
   const int warps = sp.kw * sp.rw;
   const uint32_t inbox = smem_of(smem), ring = inbox + sp.inbox + warp * (STAGES * STAGE_BYTES), xs = inbox + sp.inbox + warps * (STAGES * STAGE_BYTES);
-  const int set_bytes = Q * cv * 64, step_bytes = SETS * set_bytes;
+  const int set_bytes = Q * cv * (P == DIGITS ? 32 : 64), step_bytes = SETS * set_bytes;
+  const uint32_t factors = xs + min(sp.per_phase, share) * 4 * step_bytes;  // (digits only)
   const bool wide = w.n_in % (P == 3 ? 4 : 8) == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0;
   Stager<P, PACKED, NT, DUAL> stager;
   int to = min(first + sp.per_phase, end);
@@ -187,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
       stager.fetch(p, from, m0, wide);
     }
     while (true) {
-      stager.put(p, cv, step_bytes, set_bytes, xs);
+      stager.put(p, cv, step_bytes, set_bytes, xs, factors);
       if (stager.item - threadIdx.x >= stager.items) break;
       stager.fetch(p, from, m0, wide);
     }
@@ -199,7 +261,49 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
       const uint32_t st = ring + slot * STAGE_BYTES + g * ROW_BYTES + t * 4;
       slot = slot == STAGES - 1 ? 0 : slot + 1;
       const uint32_t sc = st - g * (ROW_BYTES - 4) - t * 4 + TILE_N * ROW_BYTES;
-      const uint32_t xb = xs + (c - from) * 4 * step_bytes + (min(g, cv - 1) * 4 + t) * 16;  // columns that are not held repeat the last
+      const int held = min(g, cv - 1);  // columns that are not held repeat the last
+      if constexpr (P == DIGITS) {
+        const uint32_t xb = xs + (c - from) * 4 * step_bytes + (held * 4 + t) * 8;
+        int acc[2][NT][4];
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          if (step % F == 0) {  // (1.5 * 2^23 as a bit pattern: a whole number added to it is that number added to 1.5 * 2^23)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[r][j][i] = 0x4B400000;
+          }
+          uint32_t b[NT][2];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(b[j][0]), "=r"(b[j][1]) : "r"(xb + step * step_bytes + j * cv * 32) : "memory");
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t w0 = lds32(st + r * 16 * ROW_BYTES + step * 16), w1 = lds32(st + (r * 16 + 8) * ROW_BYTES + step * 16);
+            const uint32_t a0 = digits_of(w0 * 16u), a1 = digits_of(w1 * 16u), a2 = digits_of(w0), a3 = digits_of(w1);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma_digits(acc[r][j], a0, a1, a2, a3, b[j][0], b[j][1]);
+          }
+          if (step % F == F - 1) {  // the group ends here
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t at = sc + (step / F) * TILE_N * 4 + r * 64;
+              const float s0 = __uint_as_float(lds32(at)), s1 = __uint_as_float(lds32(at + 32));
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                float f[2];
+                asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(f[0]), "=f"(f[1]) : "r"(factors + (((c - from) * (4 / F) + step / F) * NT * 8 + j * 8 + 2 * t) * 4) : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  tot[0][r][j][i] = fmaf((__int_as_float(acc[r][j][i]) - 12582912.f) * f[i & 1], i < 2 ? s0 : s1, tot[0][r][j][i]);
+              }
+            }
+          }
+        }
+      } else {
+      const uint32_t xb = xs + (c - from) * 4 * step_bytes + (held * 4 + t) * 16;
       float acc[SETS][2][NT][4];
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
@@ -256,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
             }
           }
         }
+      }
       }
     }
   }
@@ -326,7 +431,7 @@ int forward(const W4LinearArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
   constexpr int Q = (PACKED ? 1 : P) * NT, SETS = DUAL ? 2 : 1, COUNT = PACKED ? P : 1;
   const int tiles_n = ceil_div(p.w.n_out, TILE_N), chunks = ceil_div(p.w.n_in, CHUNK);
   const int cv = NT > 1 ? 8 : sp.tile_m * COUNT;
-  const int chunk_bytes = 4 * SETS * Q * cv * 64;
+  const int chunk_bytes = P == DIGITS ? 4 * NT * cv * 32 + 4 * NT * 32 : 4 * SETS * Q * cv * 64;
   // 16 warps an SM: the columns are split as often as that takes.  Over a cluster while a block's part of the rows is long (every block makes
   // parts of what it reads, 4096 elements take about a microsecond), else over the warps of a block.
   const long long units = (long long)tiles_n * tiles_m;
@@ -360,7 +465,8 @@ int forward(const W4LinearArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
 int launch_w4_linear(const W4LinearArgs& all, cudaStream_t stream) {
   Split sp = {};
   const bool dual = all.b != nullptr;
-  const int parts = all.type == BF_TYPE_F32 ? 3 : all.type == BF_TYPE_F16 ? 2 : 1;
+  const bool digits = all.type != BF_TYPE_F32 && all.M <= 4;
+  const int parts = digits ? DIGITS : all.type == BF_TYPE_F32 ? 3 : all.type == BF_TYPE_F16 ? 2 : 1;
   const int side = all.M * parts;  // columns that the rows' parts fill side by side: fewer instructions up to two tiles
   // (9 and 10 rows in three parts: 4 tiles side by side, 6 otherwise)
   sp.packed = side <= 8 || (side <= 16 && parts > 1) || (side > 24 && side <= 32 && parts == 3 && !dual);
@@ -380,6 +486,7 @@ int launch_w4_linear(const W4LinearArgs& all, cudaStream_t stream) {
     if (dual)
       rc = sp.packed ? (nt == 1 ? forward<3, true, 1, true>(p, sp, here, stream) : forward<3, true, 2, true>(p, sp, here, stream))
                      : (nt == 1 ? forward<3, false, 1, true>(p, sp, here, stream) : forward<3, false, 2, true>(p, sp, here, stream));
+    else if (digits) rc = nt == 1 ? forward<DIGITS, true, 1, false>(p, sp, here, stream) : forward<DIGITS, true, 2, false>(p, sp, here, stream);
     else if (parts == 3)
       rc = sp.packed ? (nt == 1 ? forward<3, true, 1, false>(p, sp, here, stream) : nt == 2 ? forward<3, true, 2, false>(p, sp, here, stream)
                                                                                             : forward<3, true, 4, false>(p, sp, here, stream))

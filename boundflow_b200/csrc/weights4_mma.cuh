@@ -53,6 +53,18 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Codes in the upper halves of the bytes, minus 8 and times 16, as four 8-bit numbers: the highest bit turned makes two's complement of them.
+__device__ __forceinline__ uint32_t digits_of(uint32_t w) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(v) : "r"(w), "r"(0xf0f0f0f0u), "r"(0x80808080u));
+  return v;
+}
+__device__ __forceinline__ void mma_digits(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // Bit patterns of two numbers to the words (first, second) of their bfloat16 parts: three parts of 8 bits, or two, the second rounded to the nearest.
 // Infinities and NaN are one part.
 __device__ __forceinline__ void one_number(float v, int parts, uint32_t (&p)[3]) {

@@ -247,6 +247,40 @@ def test_special_values(dev):
     assert float(linear4(tiny, W).abs().max()) <= 1e-35
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+def test_16_bit_rows_of_all_magnitudes(dev, kind, m):
+    """Few 16-bit rows are counted in units of 2^-30 of the largest of 128 columns: off by half a unit, beside the rounding of the result.  Magnitudes over the whole
+    range of the type, its largest and smallest, zeros, and rows of infinities and NaN."""
+    from boundflow_b200.weights4 import linear4
+
+    n, k, group = 70, 700, 64
+    W, w, g = make(n, k, group, dev, 9)
+    t = TYPES[kind]
+    span = 30 if kind == "bf16" else 5
+    x = (torch.randn(m, k, generator=g) * torch.exp2(span * torch.randn(m, k, generator=g).clamp(-3, 3))).clamp(-6e4, 6e4).to(t).to(dev)
+    x[0, :128] = torch.finfo(t).tiny / 2   # a whole chunk below the normal range
+    x[0, 128:256] = 0
+    x[m - 1, 300], x[m - 1, 301] = 60000.0, -torch.finfo(t).tiny
+    xd = x.double()
+    top = torch.nn.functional.pad(xd.abs(), (0, 68)).view(m, -1, 128).amax(2).repeat_interleave(128, dim=1)[:, :k].clamp(min=2.0 ** -97)
+    want, size = xd @ w.t(), xd.abs() @ w.abs().t()
+    got = linear4(x * 1.0, W)
+    unit = (top * 2.0 ** -30) @ w.abs().t()
+    half = torch.finfo(t).eps / 2
+    tol = unit + 2.0 ** -24 * (k / 8 + 32) * size + half * 1.01 * want.abs() + torch.finfo(t).tiny
+    fine = want.abs() <= torch.finfo(t).max
+    assert bool(((got.double() - want).abs() <= tol)[fine].all())
+    assert (got.double().abs()[~fine] >= torch.finfo(t).max).all()
+    y = x.clone()
+    y[m - 1, 17] = float("inf")
+    out, q = linear4(y, W)[m - 1], w[:, 17]
+    assert out[q == 0].isnan().all() and (out[q > 0] == float("inf")).all() and (out[q < 0] == -float("inf")).all()
+    y[m - 1, 400] = float("nan")
+    out = linear4(y, W)
+    assert out[m - 1].isnan().all() and torch.equal(out[: m - 1], got[: m - 1])
+
+
 def test_same_bits_again_and_in_a_graph(dev):
     """Fixed sums: the same call twice gives the same bits, also replayed, also beside a call on other data on another stream."""
     from boundflow_b200.weights4 import interval_linear4, linear4, rows_times_weight4
