@@ -1,6 +1,8 @@
 // Linear layers whose weights are held in 4 bits (weights4.cuh): quantisation, unpacking, the sums beside the products, and the C entries.
 #include <math.h>
 
+#include <algorithm>
+
 #include "weights4.cuh"
 
 namespace bf {
@@ -26,23 +28,27 @@ __device__ __forceinline__ void load_eight(const void* p, int type, long long at
     }
   }
 }
-// Bit pattern of the largest magnitude, that of a NaN where an infinity or a NaN is among them.
+// Bit pattern of the largest magnitude, that of a NaN where one is among them.
 __device__ __forceinline__ uint32_t largest(const float (&v)[8]) {
-  float top = 0.f, finite = 0.f;
+  float top = fabsf(v[0]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    top = fmaxf(top, fabsf(v[j]));
-    finite = fmaf(v[j], 0.f, finite);
-  }
-  return finite == 0.f ? __float_as_uint(top) : 0x7fc00000u;
+  for (int j = 1; j < 8; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[j])));
+  return __float_as_uint(top) & 0x7fffffffu;
+}
+// 1 / x to the nearest, for normal x with a normal reciprocal: the approximation is within one unit in the last place, and Newton's step in two multiply-adds rounds
+// correctly from there (Markstein 1990, who excepts a mantissa of ones; all 2^23 mantissas were compared with the division here, that one among them).
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return fmaf(fmaf(-x, y, 1.f), y, y);
 }
 // Eight codes.  The quotient is the rounded one of a division by definition: with the rounded reciprocal, a product and the remainder that it leaves give it exactly
 // (Markstein 1990).  Adding 1.5 * 2^23 rounds to a whole number and leaves it, + 8, in the last bits, which are collected with products: what the
 // constants' own bits come to is taken off at the end.  (16-bit weights lie on a lattice, halves of a code are frequent among them: no branch for those.)
-__device__ __forceinline__ uint32_t codes_of(const float (&v)[8], float scale, float inverse) {
-  if (!(scale > 0.f && scale < INFINITY)) return 0x88888888u;  // zeros, or a group that its scale makes NaN
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[8], float scale) {
   uint32_t word = 0;
-  if (scale > 1e-30f) {
+  if (scale > 1e-30f && scale < 1e30f) {
+    const float inverse = reciprocal(scale);
 #pragma unroll
     for (int j = 7; j >= 0; --j) {
       const float near = v[j] * inverse;
@@ -50,6 +56,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[8], float scale, f
     }
     return word - 0x4B400000u * 0x11111111u;
   }
+  if (!(scale > 0.f && scale < INFINITY)) return 0x88888888u;  // zeros, or a group that its scale makes NaN
 #pragma unroll
   for (int j = 7; j >= 0; --j) word = word * 16u + (uint32_t)(__float2int_rn(fminf(fmaxf(rintf(__fdiv_rn(v[j], scale)), -7.f), 7.f)) + 8);
   return word;
@@ -83,10 +90,10 @@ __device__ __forceinline__ void numbers(const Raw<__half>& w, float (&v)[8]) {
     v[2 * j + 1] = f.y;
   }
 }
-template <typename T>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) w4_quantise_kernel(const T* W, int type, uint8_t* codes, float* scales, W4 w) {
   constexpr int AHEAD = 4;
-  const int padded = w.groups() << w.group_log2, lane8 = (threadIdx.x & 31) * 8, lanes = 1 << (w.group_log2 - 3);
+  const int padded = w.groups() << w.group_log2, lane8 = (threadIdx.x & 31) * 8;
   const unsigned per_row = (unsigned)(padded + 1023) >> 10;
   const long long turns = (long long)w.n_out * per_row, stride = (long long)gridDim.x * 8;
   const bool wide = w.n_in % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
@@ -109,14 +116,22 @@ __global__ void __launch_bounds__(256) w4_quantise_kernel(const T* W, int type, 
       if (whole) numbers(raw[i], v);
       else load_eight(W, type, n * w.n_in + k0 + 256 * i, w.n_in - k0 - 256 * i, wide, v);
       uint32_t top = largest(v);
-      for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int o = LANES >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float scale = __fmul_rn(__uint_as_float(top), 1.f / 7.f);
       if (k0 + 256 * i < padded) {
-        out[32 * i] = codes_of(v, scale, __frcp_rn(scale));
-        if ((threadIdx.x & (lanes - 1)) == 0) to[(long long)((256 * i) >> w.group_log2) * w.n_out] = scale;
+        out[32 * i] = codes_of(v, scale);
+        if ((threadIdx.x & (LANES - 1)) == 0) to[(long long)((256 * i) >> w.group_log2) * w.n_out] = scale;
       }
     }
   }
+}
+template <typename T>
+void quantise(const T* W, int type, uint8_t* codes, float* scales, const W4& w, int blocks, cudaStream_t stream) {
+  if (w.group_log2 == 5) w4_quantise_kernel<T, 4><<<blocks, 256, 0, stream>>>(W, type, codes, scales, w);
+  else if (w.group_log2 == 6) w4_quantise_kernel<T, 8><<<blocks, 256, 0, stream>>>(W, type, codes, scales, w);
+  else if (w.group_log2 == 7) w4_quantise_kernel<T, 16><<<blocks, 256, 0, stream>>>(W, type, codes, scales, w);
+  else w4_quantise_kernel<T, 32><<<blocks, 256, 0, stream>>>(W, type, codes, scales, w);
 }
 // Groups over 256: a warp each, which reads it twice.
 __global__ void __launch_bounds__(256) w4_quantise_long_kernel(const void* W, int type, uint8_t* codes, float* scales, W4 w) {
@@ -134,45 +149,60 @@ __global__ void __launch_bounds__(256) w4_quantise_long_kernel(const void* W, in
     }
     const float scale = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), 1.f / 7.f);
     if (lane == 0) scales[(long long)g * w.n_out + n] = scale;
-    const float inverse = __frcp_rn(scale);
     uint32_t* out = reinterpret_cast<uint32_t*>(codes + n * w.pitch() + (long long)g * (G / 2));
     for (int j = lane * 8; j < G; j += 256) {
       load_eight(W, type, n * w.n_in + g * G + j, w.n_in - g * G - j, wide, v);
-      out[j / 8] = codes_of(v, scale, inverse);
+      out[j / 8] = codes_of(v, scale);
     }
   }
 }
 
-// code - 8 in 8 bits, or the weight in 32: eight neighbours a thread.
-__global__ void __launch_bounds__(256) w4_unpack_kernel(W4 w, int8_t* integers, float* dense) {
-  const unsigned per_row = (unsigned)((w.n_in + 7) >> 3);
+// A word's codes - 8 as eight 8-bit numbers: a byte c of 0..15 to c - 8, where (128 + c - 8) with its highest bit turned borrows nothing from its neighbour.
+__device__ __forceinline__ uint2 integers_of(uint32_t word) {
+  const uint32_t lo = (((word & 0x0f0f0f0fu) | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
+  const uint32_t hi = ((((word >> 4) & 0x0f0f0f0fu) | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
+  return make_uint2(__byte_perm(lo, hi, 0x5140), __byte_perm(lo, hi, 0x7362));
+}
+// code - 8 in 8 bits: PER columns a thread, 16 where rows are whole multiples of that.
+template <int PER>
+__global__ void __launch_bounds__(256) w4_integers_kernel(W4 w, int8_t* integers) {
+  const unsigned per_row = (unsigned)(w.n_in + PER - 1) / PER;
   const long long units = (long long)w.n_out * per_row, pitch = w.pitch();
   for (long long u = blockIdx.x * 256LL + threadIdx.x; u < units; u += gridDim.x * 256LL) {
     const long long n = units < (1LL << 32) ? (long long)((unsigned)u / per_row) : u / per_row;
-    const int k = (int)(u - n * per_row) * 8, left = min(8, w.n_in - k);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(w.codes + n * pitch + k / 2);
-    // a byte c of 0..15 to c - 8: (128 + c - 8) with its highest bit turned borrows nothing from its neighbour
-    const uint32_t lo = (((word & 0x0f0f0f0fu) | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
-    const uint32_t hi = ((((word >> 4) & 0x0f0f0f0fu) | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
-    const uint32_t q[2] = {__byte_perm(lo, hi, 0x5140), __byte_perm(lo, hi, 0x7362)};
-    const long long at = n * w.n_in + k;
-    if (integers) {
-      if (w.n_in % 8 == 0 && (reinterpret_cast<uintptr_t>(integers) & 7) == 0) {
-        *reinterpret_cast<uint2*>(integers + at) = make_uint2(q[0], q[1]);
-      } else {
-        for (int j = 0; j < left; ++j) integers[at + j] = (int8_t)(q[j >> 2] >> (8 * (j & 3)));
-      }
+    const int k = (int)(u - n * per_row) * PER;
+    int8_t* to = integers + n * w.n_in + k;
+    if (PER == 16) {
+      const uint2 words = *reinterpret_cast<const uint2*>(w.codes + n * pitch + k / 2), a = integers_of(words.x), b = integers_of(words.y);
+      *reinterpret_cast<uint4*>(to) = make_uint4(a.x, a.y, b.x, b.y);
     } else {
-      const float scale = w.scales[(long long)(k >> w.group_log2) * w.n_out + n];
-      float v[8];
+      const uint2 q = integers_of(*reinterpret_cast<const uint32_t*>(w.codes + n * pitch + k / 2));
+      const int left = min(8, w.n_in - k);
+      for (int j = 0; j < left; ++j) to[j] = (int8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+    }
+  }
+}
+// The weight in 32 bits: eight columns a thread.
+__global__ void __launch_bounds__(256) w4_dense_kernel(W4 w, float* dense) {
+  const unsigned per_row = (unsigned)((w.n_in + 7) >> 3);
+  const long long units = (long long)w.n_out * per_row, pitch = w.pitch();
+  const bool wide = w.n_in % 4 == 0 && (reinterpret_cast<uintptr_t>(dense) & 15) == 0;
+  for (long long u = blockIdx.x * 256LL + threadIdx.x; u < units; u += gridDim.x * 256LL) {
+    const long long n = units < (1LL << 32) ? (long long)((unsigned)u / per_row) : u / per_row;
+    const int k = (int)(u - n * per_row) * 8, left = min(8, w.n_in - k);
+    const uint2 q = integers_of(*reinterpret_cast<const uint32_t*>(w.codes + n * pitch + k / 2));
+    const float scale = w.scales[(long long)(k >> w.group_log2) * w.n_out + n];
+    float* to = dense + n * w.n_in + k;
+    float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = scale * (float)(int8_t)(q[j >> 2] >> (8 * (j & 3)));
-      if (w.n_in % 4 == 0 && left == 8 && (reinterpret_cast<uintptr_t>(dense) & 15) == 0) {
-        reinterpret_cast<float4*>(dense + at)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dense + at)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        for (int j = 0; j < left; ++j) dense[at + j] = v[j];
-      }
+    for (int j = 0; j < 8; ++j) v[j] = scale * (float)(int8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+    if (wide && left == 8) {
+      reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) to[j] = v[j];
     }
   }
 }
@@ -215,7 +245,7 @@ int make_w4(W4& w, const char* who, const void* codes, const void* scales, int n
 }
 
 int blocks_for(long long units, int per_block) {
-  const long long b = (units + per_block - 1) / per_block, cap = 148LL * 32;
+  const long long b = (units + per_block - 1) / per_block, cap = 148LL * 256;
   return (int)(b < cap ? b : cap);
 }
 
@@ -228,12 +258,10 @@ extern "C" int bf_w4_quantise(const void* W, int type, uint8_t* codes, float* sc
   if (rc != BF_OK) return rc;
   BF_REQUIRE(W && bf::type_ok(type), BF_E_INVALID, "bf_w4_quantise: null weight or unknown type %d", type);
   const long long turns = (long long)n_out * ((((long long)w.groups() << w.group_log2) + 1023) / 1024);
-  if (w.group_log2 <= 8) {
-    const int blocks = bf::blocks_for(turns, 8);
-    if (type == BF_TYPE_F32) bf::w4_quantise_kernel<<<blocks, 256, 0, bf::as_stream(stream)>>>(static_cast<const float*>(W), type, codes, scales, w);
-    else if (type == BF_TYPE_BF16) bf::w4_quantise_kernel<<<blocks, 256, 0, bf::as_stream(stream)>>>(static_cast<const __nv_bfloat16*>(W), type, codes, scales, w);
-    else bf::w4_quantise_kernel<<<blocks, 256, 0, bf::as_stream(stream)>>>(static_cast<const __half*>(W), type, codes, scales, w);
-  } else bf::w4_quantise_long_kernel<<<bf::blocks_for((long long)n_out * w.groups(), 8), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
+  if (w.group_log2 > 8) bf::w4_quantise_long_kernel<<<bf::blocks_for((long long)n_out * w.groups(), 8), 256, 0, bf::as_stream(stream)>>>(W, type, codes, scales, w);
+  else if (type == BF_TYPE_F32) bf::quantise(static_cast<const float*>(W), type, codes, scales, w, bf::blocks_for(turns, 8), bf::as_stream(stream));
+  else if (type == BF_TYPE_BF16) bf::quantise(static_cast<const __nv_bfloat16*>(W), type, codes, scales, w, bf::blocks_for(turns, 8), bf::as_stream(stream));
+  else bf::quantise(static_cast<const __half*>(W), type, codes, scales, w, bf::blocks_for(turns, 8), bf::as_stream(stream));
   BF_CHECK_LAUNCH("w4_quantise_kernel");
   return BF_OK;
 }
@@ -243,8 +271,11 @@ extern "C" int bf_w4_integers(const uint8_t* codes, int8_t* out, int n_out, int 
   const int rc = bf::make_w4(w, "bf_w4_integers", codes, codes, n_out, n_in, group);
   if (rc != BF_OK) return rc;
   BF_REQUIRE(out, BF_E_INVALID, "bf_w4_integers: null output");
-  bf::w4_unpack_kernel<<<bf::blocks_for(((long long)n_in + 7) / 8 * n_out, 256), 256, 0, bf::as_stream(stream)>>>(w, out, nullptr);
-  BF_CHECK_LAUNCH("w4_unpack_kernel");
+  // (a grid of 32 blocks an SM: 8192 x 8192 24 us, 44 with a block for each 2048 columns)
+  if (n_in % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
+    bf::w4_integers_kernel<16><<<std::min(bf::blocks_for((long long)n_in / 16 * n_out, 256), 148 * 32), 256, 0, bf::as_stream(stream)>>>(w, out);
+  else bf::w4_integers_kernel<8><<<std::min(bf::blocks_for(((long long)n_in + 7) / 8 * n_out, 256), 148 * 32), 256, 0, bf::as_stream(stream)>>>(w, out);
+  BF_CHECK_LAUNCH("w4_integers_kernel");
   return BF_OK;
 }
 
@@ -253,8 +284,8 @@ extern "C" int bf_w4_dense(const uint8_t* codes, const float* scales, float* out
   const int rc = bf::make_w4(w, "bf_w4_dense", codes, scales, n_out, n_in, group);
   if (rc != BF_OK) return rc;
   BF_REQUIRE(out, BF_E_INVALID, "bf_w4_dense: null output");
-  bf::w4_unpack_kernel<<<bf::blocks_for(((long long)n_in + 7) / 8 * n_out, 256), 256, 0, bf::as_stream(stream)>>>(w, nullptr, out);
-  BF_CHECK_LAUNCH("w4_unpack_kernel");
+  bf::w4_dense_kernel<<<bf::blocks_for(((long long)n_in + 7) / 8 * n_out, 256), 256, 0, bf::as_stream(stream)>>>(w, out);
+  BF_CHECK_LAUNCH("w4_dense_kernel");
   return BF_OK;
 }
 

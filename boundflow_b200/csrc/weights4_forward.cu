@@ -132,19 +132,17 @@ struct Stager {
     }
   }
   __device__ __forceinline__ void put(const W4LinearArgs& p, int cv, int step_bytes, int set_bytes, uint32_t xs, uint32_t factors) {
-    if (P == DIGITS) {
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        if (rows[i] < 0) break;
-        put_digits(raw[i][0], p.type, 4 << min(p.w.group_log2 - 5, 2), rows[i], pieces[i], step_bytes, xs, factors);
-      }
-      return;
-    }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (rows[i] < 0) break;
+      if constexpr (P == DIGITS) put_digits(raw[i][0], p.type, 4 << min(p.w.group_log2 - 5, 2), rows[i], pieces[i], step_bytes, xs, factors);
+      else put_parts(i, p, cv, step_bytes, set_bytes, xs);
+    }
+  }
+  __device__ __forceinline__ void put_parts(int i, const W4LinearArgs& p, int cv, int step_bytes, int set_bytes, uint32_t xs) {
+    {
       uint32_t o[SETS][P][4];
-      if (P == 1 || P == DIGITS) {
+      if constexpr (P == 1) {
         const uint4 v = raw[i][0].q;
         o[0][0][0] = __byte_perm(v.x, v.z, 0x5410);
         o[0][0][1] = __byte_perm(v.x, v.z, 0x7632);

@@ -52,6 +52,13 @@ class Weight4:
             raise ValueError("Weight4: codes and scales must be contiguous, codes on a 16-byte boundary")
         self.codes, self.scales, self.n_out, self.n_in, self.group = codes, scales, n_out, n_in, group
 
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, n_out: int, n_in: int, group: int) -> "Weight4":
+        """Without the checks, for tensors made to measure."""
+        w = cls.__new__(cls)
+        w.codes, w.scales, w.n_out, w.n_in, w.group = codes, scales, n_out, n_in, group
+        return w
+
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.n_out, self.n_in)
@@ -68,11 +75,10 @@ class Weight4:
 
     def integers(self) -> torch.Tensor:
         """code - 8 as int8 [n_out, n_in]."""
-        device = _device_of(self.codes)
-        w = self.to(device)
-        out = torch.empty(w.shape, dtype=torch.int8, device=device)
-        _W4_INTEGERS(device, w.codes.data_ptr(), out.data_ptr(), w.n_out, w.n_in, w.group)
-        return out.to(self.device)
+        codes = self.codes if self.codes.is_cuda else self.codes.to(_cuda_device(self.codes))
+        out = torch.empty((self.n_out, self.n_in), dtype=torch.int8, device=codes.device)
+        _W4_INTEGERS(codes.device, codes.data_ptr(), out.data_ptr(), self.n_out, self.n_in, self.group)
+        return out if self.codes.is_cuda else out.to(self.codes.device)
 
     def dense(self) -> torch.Tensor:
         """The weight in fp32."""
@@ -101,13 +107,14 @@ def quantise_weight4(W: torch.Tensor, group: int = 128) -> Weight4:
     if group < 32 or group > 1 << 20 or group & (group - 1):
         raise ValueError(f"quantise_weight4: groups of {group} weights (a power of two from 32 to 2^20 is wanted)")
     device = _device_of(W)
-    w = W.detach().to(device).contiguous()
-    n_out, n_in = int(w.shape[0]), int(w.shape[1])
+    w = _placed(W.detach() if W.requires_grad else W, device)
+    n_out, n_in = w.shape
     groups = -(-n_in // group)
     codes = torch.empty(n_out, groups * group // 2, dtype=torch.uint8, device=device)
     scales = torch.empty(groups, n_out, dtype=torch.float32, device=device)
     _W4_QUANTISE(device, w.data_ptr(), _TYPES[w.dtype], codes.data_ptr(), scales.data_ptr(), n_out, n_in, group)
-    return Weight4(codes, scales, n_in).to(W.device)
+    made = Weight4._of(codes, scales, n_out, n_in, group)
+    return made if W.is_cuda else made.to(W.device)
 
 
 # ---- launches: contiguous CUDA tensors of one device, rows [M, n] -----------------------
