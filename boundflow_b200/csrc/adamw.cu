@@ -25,6 +25,8 @@ namespace {
 constexpr int BLOCK = 256;         // elements that share an exponent: one warp's work at a time
 constexpr int CHUNK = 8 * BLOCK;   // elements of a thread block's turn
 
+constexpr int STARTS = 256;
+
 struct AdamEntry {
   void* p;
   const void* g;
@@ -39,6 +41,8 @@ struct AdamTable {
   AdamEntry e[CAP];
   int count;
   unsigned chunks;
+  int shift;             // chunk >> shift < STARTS
+  uint16_t start[STARTS];  // the tensor that the first chunk of that many belongs to: a search is a step or two from there
 };
 struct AdamCommon {
   void *m, *v;
@@ -228,17 +232,9 @@ __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_
   __shared__ float sh_rate, sh_root, sh_scale;
   __shared__ uint32_t sh_key;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int near = 0;  // the tensor of the last chunk that was looked up
   auto locate = [&](unsigned chunk, Turn<P, G>& w) {
-    if (near + 1 < tab.count && chunk >= tab.e[near + 1].chunk0) {  // the last tensor that begins at or before this chunk
-      int lo = near + 1, hi = tab.count;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (chunk >= tab.e[mid].chunk0) lo = mid;
-        else hi = mid;
-      }
-      near = lo;
-    }
+    int near = tab.start[chunk >> tab.shift];
+    while (near + 1 < tab.count && chunk >= tab.e[near + 1].chunk0) ++near;  // the last tensor that begins at or before this chunk
     const AdamEntry& e = tab.e[near];
     const long long at = (long long)(chunk - e.chunk0) * CHUNK + warp * BLOCK;
     w.entry = near;
@@ -415,6 +411,12 @@ int launch(const bf_adamw_tensor* t, int count, const AdamCommon& c, cudaStream_
   BF_REQUIRE(chunks < (1ULL << 31), BF_E_UNSUPPORTED, "bf_adamw_step: more than 2^42 elements in one launch");
   tab.count = count;
   tab.chunks = (unsigned)chunks;
+  tab.shift = 0;
+  while ((chunks >> tab.shift) >= STARTS) ++tab.shift;
+  for (int i = 0, k = 0; i < STARTS; ++i) {
+    while (k + 1 < count && tab.e[k + 1].chunk0 <= ((unsigned long long)i << tab.shift)) ++k;
+    tab.start[i] = (uint16_t)k;
+  }
   // Many more blocks than the chip holds: where each takes as many turns as any other, those of an SM come to their loads together and the memory waits with the
   // arithmetic (64 million parameters: 4 and 3 blocks an SM in one wave 279 and 212 us, 64 and 24 of them 246 and 174).  But four turns at least for the 8-bit
   // ones, whose first fetch nothing hides (3.3 million: 17.8 us with one turn each, 14.3 with four).
