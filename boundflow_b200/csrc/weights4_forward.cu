@@ -237,8 +237,7 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
     copies_begin();
     next += sp.kw;
   };
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) load_next(ring + s * STAGE_BYTES);
+  load_next(ring);  // one stage; the others when the rows are in place (issuing them takes as long as the memory takes to answer)
   int slot = 0;
   for (int from = first; from < end; from = to, to = min(from + sp.per_phase, end)) {
     if (from != first) {
@@ -250,6 +249,10 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
       stager.put(p, cv, step_bytes, set_bytes, xs, factors);
       if (stager.item - threadIdx.x >= stager.items) break;
       stager.fetch(p, from, m0, wide);
+    }
+    if (from == first) {
+#pragma unroll
+      for (int s = 1; s < STAGES - 1; ++s) load_next(ring + s * STAGE_BYTES);
     }
     __syncthreads();
     for (int c = from + kw; c < to; c += sp.kw) {
@@ -305,16 +308,6 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
       float acc[SETS][2][NT][4];
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        if (step % F == 0) {
-#pragma unroll
-          for (int s = 0; s < SETS; ++s)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[s][r][j][i] = 0.f;
-        }
         uint32_t b[SETS][Q][4];
 #pragma unroll
         for (int s = 0; s < SETS; ++s)
@@ -331,12 +324,18 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
           for (int h = 0; h < 2; ++h) {
             uint32_t a[4] = {weights_of(w0 >> (8 * h)), weights_of(w1 >> (8 * h)), weights_of(w0 >> (8 * h + 4)), weights_of(w1 >> (8 * h + 4))};
 #pragma unroll
-            for (int q = 0; q < Q; ++q) mma(acc[0][r][q % NT], a[0], a[1], a[2], a[3], b[0][q][2 * h], b[0][q][2 * h + 1]);
+            for (int q = 0; q < Q; ++q) {
+              if (step % F == 0 && h == 0 && q < NT) mma_anew(acc[0][r][q % NT], a[0], a[1], a[2], a[3], b[0][q][2 * h], b[0][q][2 * h + 1]);
+              else mma(acc[0][r][q % NT], a[0], a[1], a[2], a[3], b[0][q][2 * h], b[0][q][2 * h + 1]);
+            }
             if (DUAL) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) a[i] &= 0x7fff7fffu;
 #pragma unroll
-              for (int q = 0; q < Q; ++q) mma(acc[SETS - 1][r][q % NT], a[0], a[1], a[2], a[3], b[SETS - 1][q][2 * h], b[SETS - 1][q][2 * h + 1]);
+              for (int q = 0; q < Q; ++q) {
+                if (step % F == 0 && h == 0 && q < NT) mma_anew(acc[SETS - 1][r][q % NT], a[0], a[1], a[2], a[3], b[SETS - 1][q][2 * h], b[SETS - 1][q][2 * h + 1]);
+                else mma(acc[SETS - 1][r][q % NT], a[0], a[1], a[2], a[3], b[SETS - 1][q][2 * h], b[SETS - 1][q][2 * h + 1]);
+              }
             }
           }
         }

@@ -20,8 +20,8 @@ from .weights4 import _Entry
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 _PAIRS = {(p, g) for p in _TYPES for g in _TYPES if p == g or p == torch.float32}
 _SIZE = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}
-_GRAD, _SHAPE, _DEVICE, _DTYPE, _BYTES = (operator.attrgetter(n) for n in ("grad", "shape", "device", "dtype", "nbytes"))
-_POINTER, _CONTIGUOUS = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_GRAD, _SHAPE, _DTYPE, _BYTES = (operator.attrgetter(n) for n in ("grad", "shape", "dtype", "nbytes"))
+_POINTER, _CONTIGUOUS, _INDEX = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
 _ADAMW_STEP, _ADAMW_MOMENTS = _Entry("bf_adamw_step"), _Entry("bf_adamw_moments")
 _BLOCK = 256  # moments that share an exponent; a tensor's moments begin at a whole block
 _ENTRY = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.int64), ("first", np.int64), ("lr", np.float32), ("weight_decay", np.float32)])
@@ -74,6 +74,7 @@ class AdamW:
         self._options()
         self.betas, self.eps, self.state_bits, self.device = (b1, b2), float(eps), state_bits, self._params[0].device
         self._sizes, self._types = [p.numel() for p in self._params], [p.dtype for p in self._params]
+        self._bytes, self._one_type = [n * _SIZE[t] for n, t in zip(self._sizes, self._types)], len(set(self._types)) == 1
         self._inference = any(p.is_inference() for p in self._params)
         self._first = np.concatenate([[0], np.cumsum([-(-n // _BLOCK) * _BLOCK for n in self._sizes])]).astype(np.int64)
         total = max(_BLOCK, int(self._first[-1]))
@@ -127,23 +128,29 @@ class AdamW:
             if not live:
                 return
             moved, given, sizes, ptypes = ([xs[k] for k in live] for xs in (params, given, sizes, ptypes))
-        if grads is not None:  # (a tensor's .grad has its shape, type and device)
-            shapes = list(map(_SHAPE, moved))
-            if list(map(_SHAPE, given)) != shapes or set(map(_DEVICE, given)) != {device}:
-                k, g = next((k, g) for k, g, s in zip(live, given, shapes) if g.shape != s or g.device != device)
-                raise ValueError(f"AdamW.step: gradient {k} is {tuple(g.shape)} on {g.device}, not {tuple(params[k].shape)} on {device}")
+        index = [device.index] * len(given)
+        if list(map(_INDEX, moved)) != index:
+            raise ValueError(f"AdamW.step: a tensor has left {device}")
+        shapes = list(map(_SHAPE, moved)) if grads is not None else None  # (a tensor's .grad has its shape and type)
+        if list(map(_INDEX, given)) != index or (shapes is not None and list(map(_SHAPE, given)) != shapes):
+            k, g = next((k, g) for k, g in zip(live, given) if g.shape != params[k].shape or g.device != device)
+            raise ValueError(f"AdamW.step: gradient {k} is {tuple(g.shape)} on {g.device}, not {tuple(params[k].shape)} on {device}")
         if not all(map(_CONTIGUOUS, given)):
             if any(g.layout is not torch.strided for g in given):
                 raise ValueError("AdamW.step: gradients have to be strided tensors")
             given = [g.contiguous() for g in given]  # (copies live until the launch)
         gtypes = list(map(_DTYPE, given))
-        kinds = list(zip(ptypes, gtypes))
-        one = len(set(kinds)) == 1
-        for k, (pt, gt) in zip(live, kinds) if not one or kinds[0] not in _PAIRS else ():
+        one = self._one_type and gtypes.count(gtypes[0]) == len(gtypes)
+        kinds = [(ptypes[0], gtypes[0])] if one else list(zip(ptypes, gtypes))
+        for k, (pt, gt) in zip(live, kinds):
             if (pt, gt) not in _PAIRS:
                 raise TypeError(f"AdamW.step: gradient {k} is {gt} for a tensor of {pt}")
-        if list(map(_BYTES, moved)) != [n * _SIZE[t] for n, t in zip(sizes, ptypes)] or list(map(_BYTES, given)) != [n * _SIZE[t] for n, t in zip(sizes, gtypes)] \
-                or not all(map(_CONTIGUOUS, moved)):
+        if moved is params:
+            wanted = self._bytes
+            given_bytes = wanted if one and ptypes[0] == gtypes[0] else [n * _SIZE[t] for n, t in zip(sizes, gtypes)]
+        else:
+            wanted, given_bytes = [n * _SIZE[t] for n, t in zip(sizes, ptypes)], [n * _SIZE[t] for n, t in zip(sizes, gtypes)]
+        if list(map(_BYTES, moved)) != wanted or list(map(_BYTES, given)) != given_bytes or not all(map(_CONTIGUOUS, moved)):
             raise ValueError("AdamW.step: a tensor has changed its shape, type or strides")
         table = self._table if moved is params else self._table[live]
         table["p"], table["g"] = array.array("Q", map(_POINTER, moved)), array.array("Q", map(_POINTER, given))

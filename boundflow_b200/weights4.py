@@ -246,6 +246,15 @@ def _check_bias(name: str, bias: Any, weight: Weight4) -> None:
         raise ValueError(f"{name}: bias {tuple(bias.shape)} does not match {weight!r}")
 
 
+def _ready(x: Any, weight: Any, width: int, bias: Any) -> bool:
+    """Whether a call can go straight to its launch: rows [M, width] and bias as the kernels read them, on the weight's device, and no gradient asked for.
+    (All else takes the checks and copies below; microseconds that a small layer's kernel does not take.)"""
+    return (x.is_cuda and x.dim() == 2 and x.shape[1] == width and x.dtype in _TYPES and x.is_contiguous() and x.get_device() == weight.codes.get_device()
+            and not (x.requires_grad and torch.is_grad_enabled())
+            and (bias is None or (torch.is_tensor(bias) and bias.is_cuda and bias.dim() == 1 and bias.shape[0] == weight.n_out and bias.dtype in _TYPES and bias.is_contiguous()
+                                  and bias.get_device() == x.get_device() and not (bias.requires_grad and torch.is_grad_enabled()))))
+
+
 def _placed(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     """`t` on `device`, contiguous: itself where it is so already."""
     return t if t.is_cuda and t.device == device and t.is_contiguous() else t.to(device).contiguous()
@@ -253,6 +262,8 @@ def _placed(t: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable in x and bias."""
+    if type(weight) is Weight4 and torch.is_tensor(x) and _ready(x, weight, weight.n_in, bias):
+        return _linear(x, weight, bias)
     _check_rows("linear4", x, weight, "n_in")
     _check_bias("linear4", bias, weight)
     device = _device_of(x)
@@ -272,6 +283,9 @@ def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, 
                      relu_in: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """Bounds of x W^T + bias for lower <= x <= upper (fp32 [..., n_in]); `relu_in` clamps the input at zero first.  Differentiable once, for lower, upper
     and bias (without relu_in)."""
+    if (type(weight) is Weight4 and torch.is_tensor(lower) and torch.is_tensor(upper) and lower.dtype == upper.dtype == torch.float32 and lower.shape == upper.shape
+            and _ready(lower, weight, weight.n_in, bias) and _ready(upper, weight, weight.n_in, None) and (bias is None or bias.dtype == torch.float32)):
+        return _interval(lower, upper, _lib.IN_LOWER_UPPER, 1 if relu_in else 0, weight, bias)
     _check_rows("interval_linear4", lower, weight, "n_in")
     _check_rows("interval_linear4", upper, weight, "n_in")
     _check_bias("interval_linear4", bias, weight)
@@ -297,6 +311,8 @@ def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, 
 
 def rows_times_weight4(A: torch.Tensor, weight: Weight4) -> torch.Tensor:
     """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once): the gradient of `linear4`.  Differentiable in A."""
+    if type(weight) is Weight4 and torch.is_tensor(A) and _ready(A, weight, weight.n_out, None):
+        return _rows(A, weight)
     _check_rows("rows_times_weight4", A, weight, "n_out")
     device = _device_of(A)
     flat = A.dim() == 2

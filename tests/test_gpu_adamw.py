@@ -270,6 +270,16 @@ def test_state_round_trip_versions_and_refusals(dev, bits):
     ]:
         with pytest.raises(error):
             call()
+    moved = torch.zeros(10, device=dev)
+    left = AdamW([moved], state_bits=bits)
+    moved.data = moved.data.cpu()
+    with pytest.raises(ValueError):
+        left.step([torch.zeros(10)])
+    moved.data = torch.zeros(5, device=dev)
+    with pytest.raises(ValueError):
+        left.step([torch.zeros(5, device=dev)])
+    with pytest.raises(ValueError):
+        left.step([torch.zeros(5, device=dev).to_sparse()])
     opt.param_groups[0]["lr"] = -1.0
     with pytest.raises(ValueError):
         opt.step(grads)
