@@ -131,6 +131,7 @@ SIGNATURES = {
     "bf_w4_interval": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
     "bf_w4_rows": (_i, [_p, _i, _p, _p, _p, _i, _i, _i, _i, _p]),
     "bf_w4_interval_grad": (_i, [_p] * 6 + [_i] * 4 + [_p]),
+    "bf_w4_linear_grad": (_i, [_p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p]),
     "bf_rows_dot": (_i, [_p, _p, _p, _i, _i, _i, _p]),
     "bf_column_sums": (_i, [_p, _i, _p, _i, _i, _i, _p]),
     "bf_adamw_step": (_i, [_p, _i, _i, _i, _i, _p, _p, _p, _p, C.c_double, C.c_double, _f, _p, _p, _i, _p]),

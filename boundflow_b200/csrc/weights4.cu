@@ -231,7 +231,7 @@ bool type_ok(int t) { return t == BF_TYPE_F32 || t == BF_TYPE_BF16 || t == BF_TY
 
 int make_w4(W4& w, const char* who, const void* codes, const void* scales, int n_out, int n_in, int group) {
   BF_REQUIRE(codes && scales, BF_E_INVALID, "%s: null weight", who);
-  BF_REQUIRE(n_out > 0 && n_in > 0 && n_in <= 1 << 30, BF_E_INVALID, "%s: bad sizes %d x %d", who, n_out, n_in);
+  BF_REQUIRE(n_out > 0 && n_in > 0 && n_in <= 1 << 30 && n_out <= 1 << 30, BF_E_INVALID, "%s: bad sizes %d x %d", who, n_out, n_in);
   BF_REQUIRE(group >= 32 && group <= 1 << 20 && (group & (group - 1)) == 0, BF_E_INVALID, "%s: group %d is not a power of two from 32 to 2^20", who, group);
   BF_REQUIRE((reinterpret_cast<uintptr_t>(codes) & 15u) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0, BF_E_INVALID,
              "%s: codes must lie on a 16-byte boundary", who);
@@ -347,6 +347,15 @@ extern "C" int bf_w4_interval_grad(const float* grad_l, const float* grad_u, con
   p.z2 = z_u;
   p.M = M;
   return bf::launch_w4_rows(p, bf::as_stream(stream));
+}
+
+extern "C" int bf_w4_linear_grad(const void* grad, int type, const uint8_t* codes, const float* scales, void* grad_x, void* grad_bias, int bias_type, int M,
+                                 int n_in, int n_out, int group, bf_stream_t stream) {
+  if (grad_x) {
+    const int rc = bf_w4_rows(grad, type, codes, scales, grad_x, M, n_in, n_out, group, stream);
+    if (rc != BF_OK) return rc;
+  }
+  return grad_bias ? bf_column_sums(grad, type, grad_bias, bias_type, M, n_out, stream) : BF_OK;
 }
 
 extern "C" int bf_rows_dot(const float* A, const float* bias, float* d, int accumulate, int M, int n, bf_stream_t stream) {

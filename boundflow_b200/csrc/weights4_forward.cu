@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
   int next = first + kw;  // the chunk that is copied next
   auto load_next = [&](uint32_t at) {
     if (next < end) {
-      load_codes(at, codes + next * (CHUNK / 2), 8LL * pitch, rows, pitch - next * (CHUNK / 2), lane);
+      load_codes(at, codes + next * (CHUNK / 2), codes, 8LL * pitch, rows, pitch - next * (CHUNK / 2), lane);
       load_scales(at, w, groups, n0, next, lane);
     }
     copies_begin();

@@ -85,9 +85,8 @@ __device__ __forceinline__ void one_number(float v, int parts, uint32_t (&p)[3])
     p[1] = __float_as_uint(r) >> 16;
     p[2] = __float_as_uint(r - __uint_as_float(__float_as_uint(r) & 0xffff0000u)) >> 16;
   } else {
-    const __nv_bfloat16 h = __float2bfloat16(v);
-    p[0] = __bfloat16_as_ushort(h);
-    p[1] = __bfloat16_as_ushort(__float2bfloat16(v - __bfloat162float(h)));
+    p[0] = bits >> 16;  // (numbers that would round to infinity come here)
+    p[1] = __bfloat16_as_ushort(__float2bfloat16(v - __uint_as_float(bits & 0xffff0000u)));
     p[2] = 0;
   }
 }
@@ -109,9 +108,11 @@ __device__ __forceinline__ void two_numbers(float a, float b, uint32_t (&p)[PART
 }
 template <int PARTS>
 __device__ __forceinline__ void two_numbers_checked(float a, float b, uint32_t (&p)[PARTS]) {
-  if (fmaf(a, 0.f, b * 0.f) == 0.f) {
+  float top;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(fabsf(a)), "f"(fabsf(b)));
+  if (top < (PARTS == 3 ? __int_as_float(0x7f800000) : 3.3e38f)) {
     two_numbers<PARTS>(a, b, p);
-  } else {  // one of them is an infinity or a NaN
+  } else {  // one of them is an infinity or a NaN, or rounds to one
     uint32_t x[3], y[3];
     one_number(a, PARTS, x);
     one_number(b, PARTS, y);
@@ -134,14 +135,14 @@ struct Split {
 };
 
 // Lanes copy a stage: codes [32 rows][64 bytes], scales of the chunk's groups.  `codes` is the lane's first 16 bytes (row lane / 4, piece lane % 4),
-// `rows` how many of the tile's rows there are, `bytes` how many of the 64 lie within the codes' rows.
-__device__ __forceinline__ void load_codes(uint32_t to, const uint8_t* codes, long long pitch8, int rows, int bytes, int lane) {
+// `rows` how many of the tile's rows there are, `bytes` how many of the 64 lie within the codes' rows; `safe` stands for what is not there.
+__device__ __forceinline__ void load_codes(uint32_t to, const uint8_t* codes, const uint8_t* safe, long long pitch8, int rows, int bytes, int lane) {
   const int row = lane >> 2, piece = (lane & 3) * 16;
   const uint32_t dst = to + row * ROW_BYTES + piece;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool ok = row + 8 * j < rows && piece < bytes;
-    copy16(dst + j * 8 * ROW_BYTES, ok ? codes + j * pitch8 : codes, ok);
+    copy16(dst + j * 8 * ROW_BYTES, ok ? codes + j * pitch8 : safe, ok);
   }
 }
 __device__ __forceinline__ void load_scales(uint32_t to, const W4& w, int groups, int n0, int chunk, int lane) {
@@ -166,10 +167,10 @@ __device__ __forceinline__ void cluster_store(uint32_t at, float v, bool cluster
   if (cluster) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
   else asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 template <typename Args>

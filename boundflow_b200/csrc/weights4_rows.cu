@@ -32,8 +32,8 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
   const uint32_t place = as + ((pair >> 3) * 16 + (in8 & 3) * 4 + (in8 >> 2) * 2) * 2;
   const int size = p.type == BF_TYPE_F32 ? 4 : 2;
   const bool wide = w.n_out % 2 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & (2 * size - 1)) == 0;
-  const uint8_t* codes = w.codes + (long long)kb * (CHUNK / 2) + (lane & 3) * 16;
   const int bytes = (int)min((long long)CHUNK, pitch - (long long)kb * (CHUNK / 2));
+  const uint8_t* codes = w.codes + (long long)kb * (CHUNK / 2) + min((lane & 3) * 16, bytes - 16);
 
   float acc[SETS][4][2][NT][4];
 #pragma unroll
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
   auto load_next = [&](uint32_t to) {
     if (next < end) {
       const int n0 = next * TILE_N, rows = min(TILE_N, w.n_out - n0);
-      load_codes(to, codes + (long long)(n0 + min(lane >> 2, rows - 1)) * pitch, 8 * pitch, rows, bytes, lane);
+      const uint8_t* from = codes + (long long)(n0 + min(lane >> 2, rows - 1)) * pitch;
+      load_codes(to, from, from, 8 * pitch, rows, bytes, lane);
       load_scales(to, w, groups, n0, kb, lane);
     }
     copies_begin();

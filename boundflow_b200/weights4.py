@@ -141,6 +141,7 @@ class _Entry:
 
 
 _W4_LINEAR, _W4_INTERVAL, _W4_ROWS, _W4_INTERVAL_GRAD = (_Entry(n) for n in ("bf_w4_linear", "bf_w4_interval", "bf_w4_rows", "bf_w4_interval_grad"))
+_W4_LINEAR_GRAD = _Entry("bf_w4_linear_grad")
 _W4_QUANTISE, _W4_INTEGERS, _W4_DENSE, _COLUMN_SUMS = (_Entry(n) for n in ("bf_w4_quantise", "bf_w4_integers", "bf_w4_dense", "bf_column_sums"))
 
 
@@ -187,11 +188,16 @@ class _Linear4(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        need = ctx.needs_input_grad
+        need, w, M = ctx.needs_input_grad, ctx.weight, dy.shape[0]
         again = dy.requires_grad and torch.is_grad_enabled()  # a gradient of this gradient is asked for
         dy = dy.contiguous()
-        dx = (_Rows4.apply(dy, ctx.weight) if again else _rows(dy, ctx.weight)) if need[0] else None
-        db = (dy.float().sum(0).to(ctx.bias_type) if again else _column_sums(dy, ctx.bias_type)) if need[1] else None
+        if again or M == 0:
+            dx = (_Rows4.apply(dy, w) if again else _rows(dy, w)) if need[0] else None
+            return dx, dy.float().sum(0).to(ctx.bias_type) if need[1] else None, None
+        dx = dy.new_empty((M, w.n_in)) if need[0] else None
+        db = dy.new_empty(w.n_out, dtype=ctx.bias_type) if need[1] else None
+        _W4_LINEAR_GRAD(dy.device, dy.data_ptr(), _TYPES[dy.dtype], w.codes.data_ptr(), w.scales.data_ptr(), None if dx is None else dx.data_ptr(),
+                        None if db is None else db.data_ptr(), 0 if db is None else _TYPES[ctx.bias_type], M, w.n_in, w.n_out, w.group)
         return dx, db, None
 
 

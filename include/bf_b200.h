@@ -716,7 +716,7 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
 
 /* A 4-bit weight W [n_out, n_in]: W[n,k] = scales[k / group, n] * (code[n,k] - 8) with codes 0..15, two in a byte (low nibble = even
  * column), rows of padded / 2 bytes where padded is n_in rounded up to a whole group (what the padding holds has no effect); scales fp32
- * [padded / group, n_out], finite; group a power of two from 32 to 2^20; codes on a 16-byte boundary.  M rows, contiguous.
+ * [padded / group, n_out], finite; group a power of two from 32 to 2^20, n_out and n_in up to 2^30; codes on a 16-byte boundary.  M rows, contiguous.
  *   bf_w4_quantise       codes and scales of W (fp32 / bf16 / fp16): scale = max |w| of the group times 1/7 (as a 32-bit number), code = w / scale to the nearest (ties to
  *                        even) + 8; a group of zeros has scale 0, one with an infinity or a NaN is NaN throughout.
  *   bf_w4_integers       code - 8 as int8 [n_out, n_in];  bf_w4_dense: W as fp32 [n_out, n_in].
@@ -724,6 +724,7 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
  *   bf_w4_interval       bounds of the same over boxes, as bf_ibp_linear computes them: W c + b -/+ |W| r; in_mode BF_IN_LOWER_UPPER or
  *                        BF_IN_MID_RAD, relu_in (with BF_IN_LOWER_UPPER) clamps the input at zero first.
  *   bf_w4_rows           z [M,n_in] = a [M,n_out] W: coefficient rows pushed back through the layer, or the gradient of bf_w4_linear.
+ *   bf_w4_linear_grad    gradients of x (bf_w4_rows) and of the bias (bf_column_sums) in one call, either NULL where it is not wanted.
  *   bf_w4_interval_grad  gradients of bf_w4_interval (BF_IN_LOWER_UPPER, no relu_in) for those of its two results.
  * A sum over the codes of one group is scaled when it is complete: products of 2^124 / group and more overflow.
  *   bf_rows_dot          d [M] = (accumulate: +=) A [M,n] . bias [n]: the bias term of a coefficient row.
@@ -739,6 +740,8 @@ int bf_w4_rows(const void* a, int type, const uint8_t* codes, const float* scale
                bf_stream_t stream);
 int bf_w4_interval_grad(const float* grad_l, const float* grad_u, const uint8_t* codes, const float* scales, float* z_l, float* z_u, int M, int n_in,
                         int n_out, int group, bf_stream_t stream);
+int bf_w4_linear_grad(const void* grad, int type, const uint8_t* codes, const float* scales, void* grad_x, void* grad_bias, int bias_type, int M,
+                      int n_in, int n_out, int group, bf_stream_t stream);
 int bf_rows_dot(const float* A, const float* bias, float* d, int accumulate, int M, int n, bf_stream_t stream);
 int bf_column_sums(const void* A, int type, void* out, int out_type, int M, int n, bf_stream_t stream);
 

@@ -96,6 +96,7 @@ def test_library_refuses(lib):
     assert lib.bf_w4_interval(p, None, 0, 0, p, p, None, p, p, 1, 64, 4, 32, None) == bad
     assert lib.bf_w4_rows(p, 5, p, p, p, 1, 64, 4, 32, None) == bad
     assert lib.bf_w4_interval_grad(p, p, p, p, None, p, 1, 64, 4, 32, None) == bad
+    assert lib.bf_w4_linear_grad(p, 9, p, p, p, None, 0, 1, 64, 4, 32, None) == bad and lib.bf_w4_linear_grad(p, 0, p, p, None, p, 9, 1, 64, 4, 32, None) == bad
     assert lib.bf_w4_quantise(p, 4, p, p, 4, 64, 32, None) == bad
     assert lib.bf_w4_integers(p, None, 4, 64, 32, None) == bad
     assert lib.bf_w4_dense(p, p, None, 4, 64, 32, None) == bad
