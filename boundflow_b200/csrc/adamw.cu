@@ -227,6 +227,9 @@ struct Turn {
   int me, ve;
 };
 
+// Bounds and measurements (B200, 64 million parameters in 40 tensors).  32-bit moments: memory; fp32 parameters with bf16 gradients 248 us, 6.7 TB/s, the rate of a plain
+// copy; all in fp32 265 us.  8-bit moments of bf16 parameters: 176 us, 3.6 TB/s, the integer ALU is 68% and the issue slots 74% busy; of fp32
+// parameters 194 to 208 us.  (A thread block's chunks lie a grid apart: with them side by side it took 272 us against 172.)
 template <typename P, typename G, bool EIGHT, int CAP>
 __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_constant__ AdamTable<CAP> tab, const AdamCommon c) {
   __shared__ float sh_rate, sh_root, sh_scale;
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_
   }
 }
 
-// The values that 8-bit moments stand for, in bfloat16 (which holds them exactly: 8 exponent bits, 3 of 7 mantissa bits).
+// The values that 8-bit moments stand for, in bfloat16 (which holds them exactly: 8 exponent bits, 3 of 7 mantissa bits).  64 million: 60 us, 6.4 TB/s.
 __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* m8, const uint8_t* v8, const uint8_t* me, const uint8_t* ve, __nv_bfloat16* m,
                                                             __nv_bfloat16* v, long long n) {
   for (long long i = (blockIdx.x * 256LL + threadIdx.x) * 8; i < n; i += gridDim.x * 2048LL) {
