@@ -131,6 +131,12 @@ SIGNATURES = {
     "bf_w4_interval": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
     "bf_w4_rows": (_i, [_p, _i, _p, _p, _p, _i, _i, _i, _i, _p]),
     "bf_w4_interval_grad": (_i, [_p] * 6 + [_i] * 4 + [_p]),
+    "bf_w4_workspace_bytes": (C.c_longlong, [_i] * 3),
+    "bf_w4_many_pays": (_i, [_i] * 7),
+    "bf_w4_linear_many": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _i, _p, _p]),
+    "bf_w4_interval_many": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "bf_w4_rows_many": (_i, [_p, _i, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "bf_w4_interval_grad_many": (_i, [_p] * 6 + [_i] * 4 + [_p, _p]),
     "bf_w4_linear_grad": (_i, [_p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p]),
     "bf_rows_dot": (_i, [_p, _p, _p, _i, _i, _i, _p]),
     "bf_column_sums": (_i, [_p, _i, _p, _i, _i, _i, _p]),

@@ -219,7 +219,31 @@ __global__ void __launch_bounds__(256) rows_dot_kernel(const float* A, const flo
   if (lane == 0) d[m] = accumulate ? d[m] + s : s;
 }
 
-// out[j] = sum over rows of A[:, j], rows in order.
+// out[j] = sum over rows of A[:, j].  Many rows: a warp for every eighth, eight on their way at a time; the warps' sums in order (4096 rows of 8192 bf16: 14 us).
+__global__ void __launch_bounds__(256) column_sums_many_kernel(const void* A, int type, void* out, int out_type, int M, int n) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0.f;
+  if (j < n) {
+    int m = warp;
+    for (; m + 56 < M; m += 64) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += load_any(A, type, (long long)(m + 8 * i) * n + j);
+    }
+    for (; m < M; m += 8) s[0] += load_any(A, type, (long long)m * n + j);
+  }
+  part[warp][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  if (warp == 0 && j < n) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += part[i][lane];
+    store_any(out, out_type, j, v);
+  }
+}
+// Few rows, in order.
 __global__ void __launch_bounds__(256) column_sums_kernel(const void* A, int type, void* out, int out_type, int M, int n) {
   const int j = blockIdx.x * 256 + threadIdx.x;
   if (j >= n) return;
@@ -290,28 +314,28 @@ extern "C" int bf_w4_dense(const uint8_t* codes, const float* scales, float* out
   return BF_OK;
 }
 
-extern "C" int bf_w4_linear(const void* x, int type, const uint8_t* codes, const float* scales, const void* bias, int bias_type, void* y, int M, int n_in,
-                            int n_out, int group, bf_stream_t stream) {
-  bf::W4LinearArgs p = {};
-  const int rc = bf::make_w4(p.w, "bf_w4_linear", codes, scales, n_out, n_in, group);
+// A product's arguments, checked.
+namespace bf {
+namespace {
+int linear_args(W4LinearArgs& p, const char* who, const void* x, int type, const uint8_t* codes, const float* scales, const void* bias, int bias_type, void* y, int M, int n_in,
+                int n_out, int group) {
+  const int rc = make_w4(p.w, who, codes, scales, n_out, n_in, group);
   if (rc != BF_OK) return rc;
-  BF_REQUIRE(x && y && M > 0 && bf::type_ok(type) && (!bias || bf::type_ok(bias_type)), BF_E_INVALID, "bf_w4_linear: null tensor, no rows or unknown type");
+  BF_REQUIRE(x && y && M > 0 && type_ok(type) && (!bias || type_ok(bias_type)), BF_E_INVALID, "%s: null tensor, no rows or unknown type", who);
   p.a = x;
   p.bias = bias;
   p.y = y;
   p.type = type;
   p.bias_type = bias_type;
   p.M = M;
-  return bf::launch_w4_linear(p, bf::as_stream(stream));
+  return BF_OK;
 }
-
-extern "C" int bf_w4_interval(const float* in_a, const float* in_b, int in_mode, int relu_in, const uint8_t* codes, const float* scales, const float* bias,
-                              float* out_l, float* out_u, int M, int n_in, int n_out, int group, bf_stream_t stream) {
-  bf::W4LinearArgs p = {};
-  const int rc = bf::make_w4(p.w, "bf_w4_interval", codes, scales, n_out, n_in, group);
+int interval_args(W4LinearArgs& p, const char* who, const float* in_a, const float* in_b, int in_mode, int relu_in, const uint8_t* codes, const float* scales, const float* bias,
+                  float* out_l, float* out_u, int M, int n_in, int n_out, int group) {
+  const int rc = make_w4(p.w, who, codes, scales, n_out, n_in, group);
   if (rc != BF_OK) return rc;
-  BF_REQUIRE(in_a && in_b && out_l && out_u && M > 0, BF_E_INVALID, "bf_w4_interval: null tensor or no rows");
-  BF_REQUIRE(in_mode == BF_IN_LOWER_UPPER || (in_mode == BF_IN_MID_RAD && !relu_in), BF_E_INVALID, "bf_w4_interval: bad input mode %d", in_mode);
+  BF_REQUIRE(in_a && in_b && out_l && out_u && M > 0, BF_E_INVALID, "%s: null tensor or no rows", who);
+  BF_REQUIRE(in_mode == BF_IN_LOWER_UPPER || (in_mode == BF_IN_MID_RAD && !relu_in), BF_E_INVALID, "%s: bad input mode %d", who, in_mode);
   p.a = in_a;
   p.b = in_b;
   p.bias = bias;
@@ -320,34 +344,94 @@ extern "C" int bf_w4_interval(const float* in_a, const float* in_b, int in_mode,
   p.mode = in_mode;
   p.relu_in = relu_in;
   p.M = M;
-  return bf::launch_w4_linear(p, bf::as_stream(stream));
+  return BF_OK;
+}
+int rows_args(W4RowsArgs& p, const char* who, const void* a, const float* b, int type, const uint8_t* codes, const float* scales, void* z, float* z2, int M, int n_in, int n_out,
+              int group) {
+  const int rc = make_w4(p.w, who, codes, scales, n_out, n_in, group);
+  if (rc != BF_OK) return rc;
+  BF_REQUIRE(a && z && (z2 == nullptr) == (b == nullptr) && M > 0 && type_ok(type), BF_E_INVALID, "%s: null tensor, no rows or unknown type", who);
+  p.a = a;
+  p.b = b;
+  p.z = z;
+  p.z2 = z2;
+  p.type = type;
+  p.M = M;
+  return BF_OK;
+}
+int check_workspace(const char* who, const void* workspace, int M, int sum, int type) {
+  BF_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 127u) == 0, BF_E_INVALID, "%s: a workspace on a 128-byte boundary is wanted", who);
+  BF_REQUIRE(w4_many_bytes(M, sum, type) > 0, BF_E_UNSUPPORTED, "%s: %d rows are too many for one call", who, M);
+  return BF_OK;
+}
+}  // namespace
+}  // namespace bf
+
+extern "C" long long bf_w4_workspace_bytes(int M, int n_sum, int type) {
+  return M > 0 && n_sum > 0 && n_sum <= 1 << 30 && bf::type_ok(type) ? bf::w4_many_bytes(M, n_sum, type) : 0;
+}
+
+extern "C" int bf_w4_many_pays(int M, int n_in, int n_out, int group, int type, int backward, int pair) {
+  if (M <= 0 || n_in <= 0 || n_out <= 0 || n_in > 1 << 30 || n_out > 1 << 30 || !bf::type_ok(type)) return 0;
+  return bf::w4_many_pays(M, n_in, n_out, group, type, backward == 0, pair != 0) ? 1 : 0;
+}
+
+extern "C" int bf_w4_linear(const void* x, int type, const uint8_t* codes, const float* scales, const void* bias, int bias_type, void* y, int M, int n_in,
+                            int n_out, int group, bf_stream_t stream) {
+  bf::W4LinearArgs p = {};
+  const int rc = bf::linear_args(p, "bf_w4_linear", x, type, codes, scales, bias, bias_type, y, M, n_in, n_out, group);
+  return rc != BF_OK ? rc : bf::launch_w4_linear(p, bf::as_stream(stream));
+}
+extern "C" int bf_w4_linear_many(const void* x, int type, const uint8_t* codes, const float* scales, const void* bias, int bias_type, void* y, int M, int n_in,
+                                 int n_out, int group, void* workspace, bf_stream_t stream) {
+  bf::W4LinearArgs p = {};
+  int rc = bf::linear_args(p, "bf_w4_linear_many", x, type, codes, scales, bias, bias_type, y, M, n_in, n_out, group);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_linear_many", workspace, M, n_in, type);
+  return rc != BF_OK ? rc : bf::launch_w4_linear_many(p, workspace, bf::as_stream(stream));
+}
+
+extern "C" int bf_w4_interval(const float* in_a, const float* in_b, int in_mode, int relu_in, const uint8_t* codes, const float* scales, const float* bias,
+                              float* out_l, float* out_u, int M, int n_in, int n_out, int group, bf_stream_t stream) {
+  bf::W4LinearArgs p = {};
+  const int rc = bf::interval_args(p, "bf_w4_interval", in_a, in_b, in_mode, relu_in, codes, scales, bias, out_l, out_u, M, n_in, n_out, group);
+  return rc != BF_OK ? rc : bf::launch_w4_linear(p, bf::as_stream(stream));
+}
+extern "C" int bf_w4_interval_many(const float* in_a, const float* in_b, int in_mode, int relu_in, const uint8_t* codes, const float* scales, const float* bias,
+                                   float* out_l, float* out_u, int M, int n_in, int n_out, int group, void* workspace, bf_stream_t stream) {
+  bf::W4LinearArgs p = {};
+  int rc = bf::interval_args(p, "bf_w4_interval_many", in_a, in_b, in_mode, relu_in, codes, scales, bias, out_l, out_u, M, n_in, n_out, group);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_interval_many", workspace, M, n_in, BF_TYPE_F32);
+  return rc != BF_OK ? rc : bf::launch_w4_linear_many(p, workspace, bf::as_stream(stream));
 }
 
 extern "C" int bf_w4_rows(const void* a, int type, const uint8_t* codes, const float* scales, void* z, int M, int n_in, int n_out, int group,
                           bf_stream_t stream) {
   bf::W4RowsArgs p = {};
-  const int rc = bf::make_w4(p.w, "bf_w4_rows", codes, scales, n_out, n_in, group);
-  if (rc != BF_OK) return rc;
-  BF_REQUIRE(a && z && M > 0 && bf::type_ok(type), BF_E_INVALID, "bf_w4_rows: null tensor, no rows or unknown type");
-  p.a = a;
-  p.z = z;
-  p.type = type;
-  p.M = M;
-  return bf::launch_w4_rows(p, bf::as_stream(stream));
+  const int rc = bf::rows_args(p, "bf_w4_rows", a, nullptr, type, codes, scales, z, nullptr, M, n_in, n_out, group);
+  return rc != BF_OK ? rc : bf::launch_w4_rows(p, bf::as_stream(stream));
+}
+extern "C" int bf_w4_rows_many(const void* a, int type, const uint8_t* codes, const float* scales, void* z, int M, int n_in, int n_out, int group, void* workspace,
+                               bf_stream_t stream) {
+  bf::W4RowsArgs p = {};
+  int rc = bf::rows_args(p, "bf_w4_rows_many", a, nullptr, type, codes, scales, z, nullptr, M, n_in, n_out, group);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_rows_many", workspace, M, n_out, type);
+  return rc != BF_OK ? rc : bf::launch_w4_rows_many(p, workspace, bf::as_stream(stream));
 }
 
 extern "C" int bf_w4_interval_grad(const float* grad_l, const float* grad_u, const uint8_t* codes, const float* scales, float* z_l, float* z_u, int M,
                                    int n_in, int n_out, int group, bf_stream_t stream) {
   bf::W4RowsArgs p = {};
-  const int rc = bf::make_w4(p.w, "bf_w4_interval_grad", codes, scales, n_out, n_in, group);
-  if (rc != BF_OK) return rc;
-  BF_REQUIRE(grad_l && grad_u && z_l && z_u && M > 0, BF_E_INVALID, "bf_w4_interval_grad: null tensor or no rows");
-  p.a = grad_l;
-  p.b = grad_u;
-  p.z = z_l;
-  p.z2 = z_u;
-  p.M = M;
-  return bf::launch_w4_rows(p, bf::as_stream(stream));
+  BF_REQUIRE(grad_u && z_u, BF_E_INVALID, "bf_w4_interval_grad: null tensor");
+  const int rc = bf::rows_args(p, "bf_w4_interval_grad", grad_l, grad_u, BF_TYPE_F32, codes, scales, z_l, z_u, M, n_in, n_out, group);
+  return rc != BF_OK ? rc : bf::launch_w4_rows(p, bf::as_stream(stream));
+}
+extern "C" int bf_w4_interval_grad_many(const float* grad_l, const float* grad_u, const uint8_t* codes, const float* scales, float* z_l, float* z_u, int M,
+                                        int n_in, int n_out, int group, void* workspace, bf_stream_t stream) {
+  bf::W4RowsArgs p = {};
+  BF_REQUIRE(grad_u && z_u, BF_E_INVALID, "bf_w4_interval_grad_many: null tensor");
+  int rc = bf::rows_args(p, "bf_w4_interval_grad_many", grad_l, grad_u, BF_TYPE_F32, codes, scales, z_l, z_u, M, n_in, n_out, group);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_interval_grad_many", workspace, M, n_out, BF_TYPE_F32);
+  return rc != BF_OK ? rc : bf::launch_w4_rows_many(p, workspace, bf::as_stream(stream));
 }
 
 extern "C" int bf_w4_linear_grad(const void* grad, int type, const uint8_t* codes, const float* scales, void* grad_x, void* grad_bias, int bias_type, int M,
@@ -368,7 +452,8 @@ extern "C" int bf_rows_dot(const float* A, const float* bias, float* d, int accu
 
 extern "C" int bf_column_sums(const void* A, int type, void* out, int out_type, int M, int n, bf_stream_t stream) {
   BF_REQUIRE(A && out && M > 0 && n > 0 && bf::type_ok(type) && bf::type_ok(out_type), BF_E_INVALID, "bf_column_sums: null tensor, bad sizes or type");
-  bf::column_sums_kernel<<<bf::ceil_div(n, 256), 256, 0, bf::as_stream(stream)>>>(A, type, out, out_type, M, n);
+  if (M > 64) bf::column_sums_many_kernel<<<bf::ceil_div(n, 32), 256, 0, bf::as_stream(stream)>>>(A, type, out, out_type, M, n);
+  else bf::column_sums_kernel<<<bf::ceil_div(n, 256), 256, 0, bf::as_stream(stream)>>>(A, type, out, out_type, M, n);
   BF_CHECK_LAUNCH("column_sums_kernel");
   return BF_OK;
 }

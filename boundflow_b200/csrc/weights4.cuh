@@ -48,5 +48,10 @@ struct W4RowsArgs {
 };
 int launch_w4_linear(const W4LinearArgs& p, cudaStream_t stream);
 int launch_w4_rows(const W4RowsArgs& p, cudaStream_t stream);
+// The same for many rows, with a workspace of w4_many_bytes (0: more rows than they take).
+long long w4_many_bytes(int M, int sum, int type);
+bool w4_many_pays(int M, int n_in, int n_out, int group, int type, bool forward, bool pair);
+int launch_w4_linear_many(const W4LinearArgs& p, void* workspace, cudaStream_t stream);
+int launch_w4_rows_many(const W4RowsArgs& p, void* workspace, cudaStream_t stream);
 
 }  // namespace bf

@@ -142,15 +142,37 @@ class _Entry:
 
 _W4_LINEAR, _W4_INTERVAL, _W4_ROWS, _W4_INTERVAL_GRAD = (_Entry(n) for n in ("bf_w4_linear", "bf_w4_interval", "bf_w4_rows", "bf_w4_interval_grad"))
 _W4_LINEAR_GRAD = _Entry("bf_w4_linear_grad")
+_W4_LINEAR_MANY, _W4_INTERVAL_MANY, _W4_ROWS_MANY, _W4_INTERVAL_GRAD_MANY = (_Entry(f"bf_w4_{n}_many") for n in ("linear", "interval", "rows", "interval_grad"))
 _W4_QUANTISE, _W4_INTEGERS, _W4_DENSE, _COLUMN_SUMS = (_Entry(n) for n in ("bf_w4_quantise", "bf_w4_integers", "bf_w4_dense", "bf_column_sums"))
+
+
+_LEAST_MANY = 32  # rows from which the kernels for many are asked about
+
+
+def _many_pays(M: int, w: Weight4, dtype: torch.dtype, backward: bool, pair: bool) -> bool:
+    return bool(_lib.load().bf_w4_many_pays(M, w.n_in, w.n_out, w.group, _TYPES[dtype], backward, pair))
+
+
+def _workspace(rows: torch.Tensor, w: Weight4, backward: bool, pair: bool = False) -> Optional[torch.Tensor]:
+    """Workspace of the kernels for many rows, or None where those for few are taken."""
+    M = rows.shape[0]
+    if M < _LEAST_MANY or not _many_pays(M, w, rows.dtype, backward, pair):
+        return None
+    need = _lib.load().bf_w4_workspace_bytes(M, rows.shape[1], _TYPES[rows.dtype])
+    return torch.empty(need, dtype=torch.uint8, device=rows.device) if need else None
 
 
 def _linear(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor]) -> torch.Tensor:
     M = x.shape[0]
     y = x.new_empty((M, w.n_out))
     if M:
-        _W4_LINEAR(x.device, x.data_ptr(), _TYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                   0 if bias is None else _TYPES[bias.dtype], y.data_ptr(), M, w.n_in, w.n_out, w.group)
+        work = _workspace(x, w, False)
+        args = (x.data_ptr(), _TYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                0 if bias is None else _TYPES[bias.dtype], y.data_ptr(), M, w.n_in, w.n_out, w.group)
+        if work is None:
+            _W4_LINEAR(x.device, *args)
+        else:
+            _W4_LINEAR_MANY(x.device, *args, work.data_ptr())
     return y
 
 
@@ -158,8 +180,13 @@ def _interval(a: torch.Tensor, b: torch.Tensor, mode: int, relu_in: int, w: Weig
     M = a.shape[0]
     lower, upper = a.new_empty((M, w.n_out)), a.new_empty((M, w.n_out))
     if M:
-        _W4_INTERVAL(a.device, a.data_ptr(), b.data_ptr(), mode, relu_in, w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                     lower.data_ptr(), upper.data_ptr(), M, w.n_in, w.n_out, w.group)
+        work = _workspace(a, w, False, True)
+        args = (a.data_ptr(), b.data_ptr(), mode, relu_in, w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                lower.data_ptr(), upper.data_ptr(), M, w.n_in, w.n_out, w.group)
+        if work is None:
+            _W4_INTERVAL(a.device, *args)
+        else:
+            _W4_INTERVAL_MANY(a.device, *args, work.data_ptr())
     return lower, upper
 
 
@@ -167,7 +194,12 @@ def _rows(a: torch.Tensor, w: Weight4) -> torch.Tensor:
     M = a.shape[0]
     z = a.new_empty((M, w.n_in))
     if M:
-        _W4_ROWS(a.device, a.data_ptr(), _TYPES[a.dtype], w.codes.data_ptr(), w.scales.data_ptr(), z.data_ptr(), M, w.n_in, w.n_out, w.group)
+        work = _workspace(a, w, True)
+        args = (a.data_ptr(), _TYPES[a.dtype], w.codes.data_ptr(), w.scales.data_ptr(), z.data_ptr(), M, w.n_in, w.n_out, w.group)
+        if work is None:
+            _W4_ROWS(a.device, *args)
+        else:
+            _W4_ROWS_MANY(a.device, *args, work.data_ptr())
     return z
 
 
@@ -191,9 +223,10 @@ class _Linear4(torch.autograd.Function):
         need, w, M = ctx.needs_input_grad, ctx.weight, dy.shape[0]
         again = dy.requires_grad and torch.is_grad_enabled()  # a gradient of this gradient is asked for
         dy = dy.contiguous()
-        if again or M == 0:
-            dx = (_Rows4.apply(dy, w) if again else _rows(dy, w)) if need[0] else None
-            return dx, dy.float().sum(0).to(ctx.bias_type) if need[1] else None, None
+        if again:
+            return _Rows4.apply(dy, w) if need[0] else None, dy.float().sum(0).to(ctx.bias_type) if need[1] else None, None
+        if M == 0 or M >= _LEAST_MANY:
+            return _rows(dy, w) if need[0] else None, _column_sums(dy, ctx.bias_type) if need[1] else None, None
         dx = dy.new_empty((M, w.n_in)) if need[0] else None
         db = dy.new_empty(w.n_out, dtype=ctx.bias_type) if need[1] else None
         _W4_LINEAR_GRAD(dy.device, dy.data_ptr(), _TYPES[dy.dtype], w.codes.data_ptr(), w.scales.data_ptr(), None if dx is None else dx.data_ptr(),
@@ -230,7 +263,12 @@ class _Interval4(torch.autograd.Function):
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
             gl, gu = dl.new_empty((M, w.n_in)), dl.new_empty((M, w.n_in))
             if M:
-                _W4_INTERVAL_GRAD(dl.device, dl.data_ptr(), du.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gl.data_ptr(), gu.data_ptr(), M, w.n_in, w.n_out, w.group)
+                work = _workspace(dl, w, True, True)
+                args = (dl.data_ptr(), du.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gl.data_ptr(), gu.data_ptr(), M, w.n_in, w.n_out, w.group)
+                if work is None:
+                    _W4_INTERVAL_GRAD(dl.device, *args)
+                else:
+                    _W4_INTERVAL_GRAD_MANY(dl.device, *args, work.data_ptr())
         if ctx.needs_input_grad[2]:
             db = _column_sums(dl, torch.float32) + _column_sums(du, torch.float32)
         return gl, gu, db, None

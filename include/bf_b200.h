@@ -726,9 +726,13 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
  *   bf_w4_rows           z [M,n_in] = a [M,n_out] W: coefficient rows pushed back through the layer, or the gradient of bf_w4_linear.
  *   bf_w4_linear_grad    gradients of x (bf_w4_rows) and of the bias (bf_column_sums) in one call, either NULL where it is not wanted.
  *   bf_w4_interval_grad  gradients of bf_w4_interval (BF_IN_LOWER_UPPER, no relu_in) for those of its two results.
+ *   *_many               the same for many rows, on the tensor cores' large tiles, with a workspace of bf_w4_workspace_bytes(M, length of the sum: n_in, or n_out for rows and
+ *                        gradients, type) bytes on a 128-byte boundary (0: more rows than one call takes, 64 * 65535).  Its first int is zero afterwards; where it is not, a
+ *                        wait on the device ran out and the results concerned are NaN.
+ *   bf_w4_many_pays      whether that is expected to be faster for these sizes (backward: rows and gradients; pair: interval and its gradient).
  * A sum over the codes of one group is scaled when it is complete: products of 2^124 / group and more overflow.
  *   bf_rows_dot          d [M] = (accumulate: +=) A [M,n] . bias [n]: the bias term of a coefficient row.
- *   bf_column_sums       out [n] = sum over the M rows of A, in order: the gradient of a bias. */
+ *   bf_column_sums       out [n] = sum over the M rows of A, in a fixed order: the gradient of a bias. */
 int bf_w4_quantise(const void* W, int type, uint8_t* codes, float* scales, int n_out, int n_in, int group, bf_stream_t stream);
 int bf_w4_integers(const uint8_t* codes, int8_t* out, int n_out, int n_in, int group, bf_stream_t stream);
 int bf_w4_dense(const uint8_t* codes, const float* scales, float* out, int n_out, int n_in, int group, bf_stream_t stream);
@@ -740,6 +744,16 @@ int bf_w4_rows(const void* a, int type, const uint8_t* codes, const float* scale
                bf_stream_t stream);
 int bf_w4_interval_grad(const float* grad_l, const float* grad_u, const uint8_t* codes, const float* scales, float* z_l, float* z_u, int M, int n_in,
                         int n_out, int group, bf_stream_t stream);
+long long bf_w4_workspace_bytes(int M, int n_sum, int type);
+int bf_w4_many_pays(int M, int n_in, int n_out, int group, int type, int backward, int pair);
+int bf_w4_linear_many(const void* x, int type, const uint8_t* codes, const float* scales, const void* bias, int bias_type, void* y, int M, int n_in,
+                      int n_out, int group, void* workspace, bf_stream_t stream);
+int bf_w4_interval_many(const float* in_a, const float* in_b, int in_mode, int relu_in, const uint8_t* codes, const float* scales, const float* bias,
+                        float* out_l, float* out_u, int M, int n_in, int n_out, int group, void* workspace, bf_stream_t stream);
+int bf_w4_rows_many(const void* a, int type, const uint8_t* codes, const float* scales, void* z, int M, int n_in, int n_out, int group, void* workspace,
+                    bf_stream_t stream);
+int bf_w4_interval_grad_many(const float* grad_l, const float* grad_u, const uint8_t* codes, const float* scales, float* z_l, float* z_u, int M,
+                             int n_in, int n_out, int group, void* workspace, bf_stream_t stream);
 int bf_w4_linear_grad(const void* grad, int type, const uint8_t* codes, const float* scales, void* grad_x, void* grad_bias, int bias_type, int M,
                       int n_in, int n_out, int group, bf_stream_t stream);
 int bf_rows_dot(const float* A, const float* bias, float* d, int accumulate, int M, int n, bf_stream_t stream);
