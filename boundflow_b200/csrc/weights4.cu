@@ -359,9 +359,8 @@ int rows_args(W4RowsArgs& p, const char* who, const void* a, const float* b, int
   p.M = M;
   return BF_OK;
 }
-int check_workspace(const char* who, const void* workspace, int M, int sum, int type) {
+int check_workspace(const char* who, const void* workspace) {
   BF_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 127u) == 0, BF_E_INVALID, "%s: a workspace on a 128-byte boundary is wanted", who);
-  BF_REQUIRE(w4_many_bytes(M, sum, type) > 0, BF_E_UNSUPPORTED, "%s: %d rows are too many for one call", who, M);
   return BF_OK;
 }
 }  // namespace
@@ -386,7 +385,7 @@ extern "C" int bf_w4_linear_many(const void* x, int type, const uint8_t* codes, 
                                  int n_out, int group, void* workspace, bf_stream_t stream) {
   bf::W4LinearArgs p = {};
   int rc = bf::linear_args(p, "bf_w4_linear_many", x, type, codes, scales, bias, bias_type, y, M, n_in, n_out, group);
-  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_linear_many", workspace, M, n_in, type);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_linear_many", workspace);
   return rc != BF_OK ? rc : bf::launch_w4_linear_many(p, workspace, bf::as_stream(stream));
 }
 
@@ -400,7 +399,7 @@ extern "C" int bf_w4_interval_many(const float* in_a, const float* in_b, int in_
                                    float* out_l, float* out_u, int M, int n_in, int n_out, int group, void* workspace, bf_stream_t stream) {
   bf::W4LinearArgs p = {};
   int rc = bf::interval_args(p, "bf_w4_interval_many", in_a, in_b, in_mode, relu_in, codes, scales, bias, out_l, out_u, M, n_in, n_out, group);
-  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_interval_many", workspace, M, n_in, BF_TYPE_F32);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_interval_many", workspace);
   return rc != BF_OK ? rc : bf::launch_w4_linear_many(p, workspace, bf::as_stream(stream));
 }
 
@@ -414,7 +413,7 @@ extern "C" int bf_w4_rows_many(const void* a, int type, const uint8_t* codes, co
                                bf_stream_t stream) {
   bf::W4RowsArgs p = {};
   int rc = bf::rows_args(p, "bf_w4_rows_many", a, nullptr, type, codes, scales, z, nullptr, M, n_in, n_out, group);
-  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_rows_many", workspace, M, n_out, type);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_rows_many", workspace);
   return rc != BF_OK ? rc : bf::launch_w4_rows_many(p, workspace, bf::as_stream(stream));
 }
 
@@ -430,7 +429,7 @@ extern "C" int bf_w4_interval_grad_many(const float* grad_l, const float* grad_u
   bf::W4RowsArgs p = {};
   BF_REQUIRE(grad_u && z_u, BF_E_INVALID, "bf_w4_interval_grad_many: null tensor");
   int rc = bf::rows_args(p, "bf_w4_interval_grad_many", grad_l, grad_u, BF_TYPE_F32, codes, scales, z_l, z_u, M, n_in, n_out, group);
-  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_interval_grad_many", workspace, M, n_out, BF_TYPE_F32);
+  if (rc == BF_OK) rc = bf::check_workspace("bf_w4_interval_grad_many", workspace);
   return rc != BF_OK ? rc : bf::launch_w4_rows_many(p, workspace, bf::as_stream(stream));
 }
 

@@ -48,7 +48,7 @@ struct W4RowsArgs {
 };
 int launch_w4_linear(const W4LinearArgs& p, cudaStream_t stream);
 int launch_w4_rows(const W4RowsArgs& p, cudaStream_t stream);
-// The same for many rows, with a workspace of w4_many_bytes (0: more rows than they take).
+// The same for many rows, with a workspace of w4_many_bytes; whether they are the faster ones.
 long long w4_many_bytes(int M, int sum, int type);
 bool w4_many_pays(int M, int n_in, int n_out, int group, int type, bool forward, bool pair);
 int launch_w4_linear_many(const W4LinearArgs& p, void* workspace, cudaStream_t stream);

@@ -129,7 +129,7 @@ struct ImageArgs {
 template <int PARTS, bool FORWARD>
 __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) {
   const long long row_eights = (long long)p.steps * 8, rows = (long long)((p.M + p.tile_m - 1) / p.tile_m) * p.tile_m, total = rows * row_eights;
-  if (FORWARD && blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
+  if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
   const bool wide = p.n % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) == 0;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
     const long long m = i / row_eights;
@@ -613,28 +613,46 @@ int launch_rows(const ManyArgs& p, int tile_m, dim3 grid, cudaStream_t stream) {
   return tile_m == 128 ? launch_unit<XP, WP, 64>(p, grid, stream) : launch_unit<XP, WP, 32>(p, grid, stream);
 }
 
+// Rows of one launch: their images are kept to 256 MB, more rows go slab by slab through the same workspace.
+int slab_of(int M, int sum, int type) {
+  const long long row = (long long)steps_of(sum) * 128 * parts_of(type), most = std::max(1LL, (256LL << 20) / row / 256) * 256;
+  return (int)std::min<long long>({M, most, 64LL * 65535});
+}
 template <bool FORWARD>
-int pass(ManyArgs p, int mode, int relu_in, void* workspace, cudaStream_t stream) {
-  const int sum = FORWARD ? p.w.n_in : p.w.n_out, features = FORWARD ? p.w.n_out : p.w.n_in, tile_m = rows_of_block(p.M, features), parts = parts_of(p.type);
+int pass(const ManyArgs& all, int mode, int relu_in, void* workspace, bool first_pass, cudaStream_t stream) {
+  const int sum = FORWARD ? all.w.n_in : all.w.n_out, features = FORWARD ? all.w.n_out : all.w.n_in, parts = parts_of(all.type), slab = slab_of(all.M, sum, all.type);
+  const int size = all.type == BF_TYPE_F32 ? 4 : 2;
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  p.steps = steps_of(sum);
-  p.status = reinterpret_cast<int*>(base);
-  p.odd = base + HEADER;
-  p.images = base + header_of(p.M);
-  ImageArgs im = {p.a, p.b, base + header_of(p.M), base + HEADER, p.status, p.type, p.take, mode, relu_in, p.M, sum, tile_m, p.steps};
-  if (!FORWARD && cudaMemsetAsync(base, 0, header_of(p.M), stream) != cudaSuccess) {
-    set_error("w4_rows_images_kernel: cannot clear the workspace");
-    return BF_E_CUDA;
+  for (long long done = 0; done < all.M; done += slab) {
+    ManyArgs p = all;
+    p.M = (int)std::min<long long>(slab, all.M - done);
+    p.a = static_cast<const char*>(all.a) + done * sum * size;
+    p.b = all.b ? all.b + done * sum : nullptr;
+    p.out = static_cast<char*>(all.out) + done * features * size;
+    p.out2 = all.out2 ? all.out2 + done * features : nullptr;
+    p.steps = steps_of(sum);
+    p.status = reinterpret_cast<int*>(base);
+    p.odd = base + HEADER;
+    p.images = base + header_of(slab);
+    const int tile_m = rows_of_block(p.M, features);
+    const ImageArgs im = {p.a, p.b, base + header_of(slab), base + HEADER, first_pass && done == 0 ? p.status : nullptr, p.type, p.take, mode, relu_in, p.M, sum, tile_m, p.steps};
+    if (!FORWARD && cudaMemsetAsync(base + HEADER, 0, p.M, stream) != cudaSuccess) {
+      set_error("w4_rows_images_kernel: cannot clear the workspace");
+      return BF_E_CUDA;
+    }
+    const long long eights = (long long)ceil_div(p.M, tile_m) * tile_m * p.steps * 8;
+    const int blocks = (int)std::min<long long>((eights + 255) / 256, 148 * 64);
+    if (parts == 1) w4_rows_images_kernel<1, FORWARD><<<blocks, 256, 0, stream>>>(im);
+    else if (parts == 2) w4_rows_images_kernel<2, FORWARD><<<blocks, 256, 0, stream>>>(im);
+    else w4_rows_images_kernel<3, FORWARD><<<blocks, 256, 0, stream>>>(im);
+    BF_CHECK_LAUNCH("w4_rows_images_kernel");
+    const dim3 grid(ceil_div(features, LANES), ceil_div(p.M, tile_m));
+    int rc;
+    if constexpr (FORWARD) rc = parts == 1 ? launch_rows<1, 1>(p, tile_m, grid, stream) : parts == 2 ? launch_rows<2, 1>(p, tile_m, grid, stream) : launch_rows<3, 1>(p, tile_m, grid, stream);
+    else rc = parts == 1 ? launch_rows<1, 2>(p, tile_m, grid, stream) : parts == 2 ? launch_rows<2, 2>(p, tile_m, grid, stream) : launch_rows<3, 3>(p, tile_m, grid, stream);
+    if (rc != BF_OK) return rc;
   }
-  const long long eights = (long long)ceil_div(p.M, tile_m) * tile_m * p.steps * 8;
-  const int blocks = (int)std::min<long long>((eights + 255) / 256, 148 * 64);
-  if (parts == 1) w4_rows_images_kernel<1, FORWARD><<<blocks, 256, 0, stream>>>(im);
-  else if (parts == 2) w4_rows_images_kernel<2, FORWARD><<<blocks, 256, 0, stream>>>(im);
-  else w4_rows_images_kernel<3, FORWARD><<<blocks, 256, 0, stream>>>(im);
-  BF_CHECK_LAUNCH("w4_rows_images_kernel");
-  const dim3 grid(ceil_div(features, LANES), ceil_div(p.M, tile_m));
-  if constexpr (FORWARD) return parts == 1 ? launch_rows<1, 1>(p, tile_m, grid, stream) : parts == 2 ? launch_rows<2, 1>(p, tile_m, grid, stream) : launch_rows<3, 1>(p, tile_m, grid, stream);
-  else return parts == 1 ? launch_rows<1, 2>(p, tile_m, grid, stream) : parts == 2 ? launch_rows<2, 2>(p, tile_m, grid, stream) : launch_rows<3, 3>(p, tile_m, grid, stream);
+  return BF_OK;
 }
 
 }  // namespace
@@ -644,8 +662,7 @@ int pass(ManyArgs p, int mode, int relu_in, void* workspace, cudaStream_t stream
 // Measured (us, many / few): 64 bf16 rows through 8192 x 4096 30.5 / 32.8, 48 fp32 ones 40.9 / 56.3, boxes of 48 82 / 122; 256 bf16 rows through 2048 x 2048
 // 21.3 / 19.8, 512 22.0 / 33.4; 1024 through 512 x 784 22.1 / 14.1; back through 8192 x 4096 128 bf16 rows 130 / 103, 192 131 / 162, 256 fp32 ones 267 / 228, 512 275 / 396.
 bool w4_many_pays(int M, int n_in, int n_out, int group, int type, bool forward, bool pair) {
-  if (w4_many_bytes(M, forward ? n_in : n_out, type) == 0) return false;
-  const int features = forward ? n_out : n_in, tile = rows_of_block(M, features), parts = parts_of(type);
+  const int features = forward ? n_out : n_in, tile = rows_of_block(slab_of(M, forward ? n_in : n_out, type), features), parts = parts_of(type);
   const double few = 4.0 + 1e-9 * M * (double)n_in * n_out * (forward ? (pair ? 55.0 : parts == 1 ? 13.5 : parts == 2 ? 18.0 : 24.0) : (pair ? 60.0 : parts == 3 ? 27.0 : 24.0));
   const double waves = (double)ceil_div((long long)ceil_div(features, LANES) * ceil_div(M, tile), 148);
   const double large = tile == 256 ? 1.0 : tile == 128 ? 0.15 : 0.0;
@@ -656,9 +673,8 @@ bool w4_many_pays(int M, int n_in, int n_out, int group, int type, bool forward,
 }
 
 long long w4_many_bytes(int M, int sum, int type) {
-  if (ceil_div(M, 64) > 65535) return 0;  // (of a grid's second axis)
-  const long long rows = (long long)ceil_div(M, 256) * 256;  // enough for blocks of any size
-  return (long long)header_of(M) + rows * steps_of(sum) * 128 * parts_of(type);
+  const int slab = slab_of(M, sum, type);
+  return (long long)header_of(slab) + (long long)ceil_div(slab, 256) * 256 * steps_of(sum) * 128 * parts_of(type);  // enough for blocks of any size
 }
 int launch_w4_linear_many(const W4LinearArgs& l, void* workspace, cudaStream_t stream) {
   ManyArgs p = {};
@@ -671,11 +687,11 @@ int launch_w4_linear_many(const W4LinearArgs& l, void* workspace, cudaStream_t s
   p.bias_type = l.bias_type;
   p.M = l.M;
   p.take = l.b ? TAKE_CENTRE : TAKE_ROWS;
-  const int rc = pass<true>(p, l.mode, l.relu_in, workspace, stream);
+  const int rc = pass<true>(p, l.mode, l.relu_in, workspace, true, stream);
   if (rc != BF_OK || !l.b) return rc;
   p.take = TAKE_RADIUS;
   p.out2 = l.y2;
-  return pass<true>(p, l.mode, l.relu_in, workspace, stream);
+  return pass<true>(p, l.mode, l.relu_in, workspace, false, stream);
 }
 int launch_w4_rows_many(const W4RowsArgs& r, void* workspace, cudaStream_t stream) {
   ManyArgs p = {};
@@ -686,11 +702,11 @@ int launch_w4_rows_many(const W4RowsArgs& r, void* workspace, cudaStream_t strea
   p.type = r.type;
   p.M = r.M;
   p.take = r.b ? TAKE_SUM : TAKE_ROWS;
-  const int rc = pass<false>(p, 0, 0, workspace, stream);
+  const int rc = pass<false>(p, 0, 0, workspace, true, stream);
   if (rc != BF_OK || !r.b) return rc;
   p.take = TAKE_DIFFERENCE;
   p.out2 = r.z2;
-  return pass<false>(p, 0, 0, workspace, stream);
+  return pass<false>(p, 0, 0, workspace, false, stream);
 }
 
 }  // namespace bf

@@ -7,7 +7,7 @@
 // 32-bit number exactly (8 + 8 + 8 bits), a 16-bit one in one part (bf16) or two (fp16).  So every product is exact and only the sums round.  The rows are
 // the instruction's 8 columns: parts side by side where that takes fewer instructions, else one instruction for each part and 8 rows.  The 128-row
 // tiles of the tcgen05 instructions would take operands through shared memory: 2 bytes a weight written and read there
-// where these kernels move half a byte, for rows that fill an eighth of the instruction's smallest tile.
+// where these kernels move half a byte, for rows that fill an eighth of the instruction's smallest tile; for many rows that is what weights4_many.cu does.
 //
 // Codes and scales come by cp.async into a ring of each warp's own (no barrier between warps), 32 rows x 128 columns a stage.
 #pragma once

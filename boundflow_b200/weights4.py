@@ -158,8 +158,7 @@ def _workspace(rows: torch.Tensor, w: Weight4, backward: bool, pair: bool = Fals
     M = rows.shape[0]
     if M < _LEAST_MANY or not _many_pays(M, w, rows.dtype, backward, pair):
         return None
-    need = _lib.load().bf_w4_workspace_bytes(M, rows.shape[1], _TYPES[rows.dtype])
-    return torch.empty(need, dtype=torch.uint8, device=rows.device) if need else None
+    return torch.empty(_lib.load().bf_w4_workspace_bytes(M, rows.shape[1], _TYPES[rows.dtype]), dtype=torch.uint8, device=rows.device)
 
 
 def _linear(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor]) -> torch.Tensor:

@@ -727,7 +727,7 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
  *   bf_w4_linear_grad    gradients of x (bf_w4_rows) and of the bias (bf_column_sums) in one call, either NULL where it is not wanted.
  *   bf_w4_interval_grad  gradients of bf_w4_interval (BF_IN_LOWER_UPPER, no relu_in) for those of its two results.
  *   *_many               the same for many rows, on the tensor cores' large tiles, with a workspace of bf_w4_workspace_bytes(M, length of the sum: n_in, or n_out for rows and
- *                        gradients, type) bytes on a 128-byte boundary (0: more rows than one call takes, 64 * 65535).  Its first int is zero afterwards; where it is not, a
+ *                        gradients, type) bytes (about 256 MB at most, or what 256 rows need; 0 for sizes or types that there are none of) on a 128-byte boundary.  Its first int is zero afterwards; where it is not, a
  *                        wait on the device ran out and the results concerned are NaN.
  *   bf_w4_many_pays      whether that is expected to be faster for these sizes (backward: rows and gradients; pair: interval and its gradient).
  * A sum over the codes of one group is scaled when it is complete: products of 2^124 / group and more overflow.

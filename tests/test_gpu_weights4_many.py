@@ -214,8 +214,12 @@ def test_refusals(dev):
     p = t.data_ptr()
     assert lib.bf_w4_linear_many(p, 0, p, p, None, 0, p, 64, 32, 4, 32, None, None) == _lib.BF_E_INVALID      # no workspace
     assert lib.bf_w4_linear_many(p, 0, p, p, None, 0, p, 64, 32, 4, 32, p + 64, None) == _lib.BF_E_INVALID    # its boundary
-    assert lib.bf_w4_rows_many(p, 0, p, p, p, 64 * 65536, 32, 4, 32, p, None) != 0                            # too many rows
-    assert lib.bf_w4_workspace_bytes(64 * 65536, 32, 0) == 0 and lib.bf_w4_workspace_bytes(64, 32, 9) == 0
+    assert lib.bf_w4_rows_many(p, 0, p, p, p, 0, 32, 4, 32, p, None) == _lib.BF_E_INVALID                     # no rows
+    assert lib.bf_w4_interval_many(p, p, 2, 0, p, p, None, p, p, 64, 32, 4, 32, p, None) == _lib.BF_E_INVALID  # unknown mode
+    assert lib.bf_w4_interval_grad_many(p, None, p, p, p, p, 64, 32, 4, 32, p, None) == _lib.BF_E_INVALID
+    assert lib.bf_w4_workspace_bytes(64, 32, 9) == 0 and lib.bf_w4_workspace_bytes(0, 32, 0) == 0
+    assert 0 < lib.bf_w4_workspace_bytes(2 ** 31 - 1, 2 ** 14, 0) < 2 ** 29
+    assert 256 * 2 ** 20 * 6 < lib.bf_w4_workspace_bytes(2 ** 31 - 1, 2 ** 20, 0) < 257 * 2 ** 20 * 6  # (256 rows at least)
     assert [lib.bf_w4_many_pays(m, 8192, 8192, 128, 1, 0, 0) for m in (0, 1, 16, 4096)] == [0, 0, 0, 1]
 
 
@@ -242,3 +246,28 @@ def test_column_sums_of_many_rows(dev):
     for m, n in ((65, 1), (64, 40), (127, 33), (128, 500), (1000, 129)):
         a = torch.randn(m, n, generator=g).to(dev)
         check(weights4._column_sums(a, torch.float32), a.double().sum(0), a.double().abs().sum(0), m, torch.float32)
+
+
+def test_more_rows_than_the_workspace_holds(dev):
+    """Slab by slab through one workspace: rows at the ends of the first and second slab, an infinity in the second."""
+    from boundflow_b200 import _lib, weights4
+
+    W, w, g = make(40, 4096, 128, dev, 10)
+    m = 12000  # 4096 columns in three parts: 24 KB a row, 10752 rows a slab
+    assert _lib.load().bf_w4_workspace_bytes(m, 4096, 0) < m * 4096 * 6
+    x = torch.randn(m, 4096, generator=g).to(dev)
+    picked = torch.tensor([0, 1, 10495, 10751, 10752, 10753, 11000, m - 1], device=dev)
+    xd = x[picked].double()
+    check(weights4.linear4(x, W)[picked], xd @ w.t(), xd.abs() @ w.abs().t(), 4096, torch.float32)
+    lower, upper = weights4.interval_linear4(x - 0.5, x + 0.5, W)
+    l, u = (x - 0.5)[picked].double(), (x + 0.5)[picked].double()
+    plus, minus = w.clamp(min=0), w.clamp(max=0)
+    check(lower[picked], l @ plus.t() + u @ minus.t(), (l.abs() + u.abs()) @ w.abs().t(), 4096, torch.float32)
+    check(upper[picked], u @ plus.t() + l @ minus.t(), (l.abs() + u.abs()) @ w.abs().t(), 4096, torch.float32)
+    V, v, g = make(4096, 40, 32, dev, 11)
+    x[11000, 17] = float("inf")
+    z = weights4.rows_times_weight4(x, V)[picked]
+    want = x[picked].double() @ v
+    keep = torch.tensor([True] * 6 + [False, True], device=dev)
+    check(z[keep], want[keep], xd[keep].abs() @ v.abs(), 4096, torch.float32)
+    assert torch.equal(torch.isnan(z[~keep]), torch.isnan(want[~keep])) and torch.equal(z[~keep].double()[torch.isinf(want[~keep])], want[~keep][torch.isinf(want[~keep])])
