@@ -14,11 +14,11 @@
 //
 // Waits are bounded: where one runs out, the block raises the status word, frees its tensor memory and stores NaN.
 //
-// Bounds and measurements (B200, images included).  4096 bf16 rows through 8192 x 4096: 328 us, 838 TFLOP/s (half of the measured rate of a library's plain product); fp32 rows, three
-// products for one, 624 us (1320 TFLOP/s of bfloat16 products); back, bf16 637 us (two products: 862), fp32 1432 us (six: 1150).  Of a stage of x W^T with 256 bf16 rows (512 clocks of
+// Bounds and measurements (B200, images included).  4096 bf16 rows through 8192 x 4096: 319 us, 861 TFLOP/s (half of the measured rate of a library's plain product); fp32 rows, three
+// products for one, 624 us (1320 TFLOP/s of bfloat16 products); back, bf16 637 us (two products: 862), fp32 1415 us (six: 1165).  Of a stage of x W^T with 256 bf16 rows (512 clocks of
 // products) 950 clocks are taken: eight warps need 730 of them for their sums, unpacking 570, issuing 380; beginning and end of a block are another 5 us that nothing hides.  Back, three pairs unpack a
 // stage in 1300 clocks and hold its slot meanwhile.  What was tried: the products issued by a thread that also unpacks (twice the time), by a thread chosen by its number instead of
-// elect.sync (41 us for 64 rows, 31 now), eight warps that both unpack and sum (528 us for 4096 rows, 328 now).
+// elect.sync (41 us for 64 rows, 31 now), eight warps that both unpack and sum (528 us for 4096 rows, 319 now).
 #include <math.h>
 
 #include <algorithm>
@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) 
   if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
   const bool wide = p.n % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) == 0;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const long long m = i / row_eights;
-    const int eight = (int)(i - m * row_eights), n = eight * 8, r = (int)(m % p.tile_m);
+    const long long m = total < (1LL << 32) ? (long long)((unsigned)i / (unsigned)row_eights) : i / row_eights;
+    const int eight = (int)(i - m * row_eights), n = eight * 8, r = (int)m & (p.tile_m - 1);  // (tiles of 64, 128 or 256)
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) 
         }
       }
     }
-    uint8_t* to = p.images + (((m / p.tile_m) * p.steps + (eight >> 3)) * PARTS * p.tile_m + r) * 128 + (((eight & 7) ^ (r & 7)) << 4);
+    uint8_t* to = p.images + ((((long long)((unsigned)m >> (31 - __clz(p.tile_m)))) * p.steps + (eight >> 3)) * PARTS * p.tile_m + r) * 128 + (((eight & 7) ^ (r & 7)) << 4);
 #pragma unroll
     for (int k = 0; k < PARTS; ++k) *reinterpret_cast<uint4*>(to + (long long)k * p.tile_m * 128) = make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
   }
