@@ -353,7 +353,8 @@ def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, 
 
 
 def rows_times_weight4(A: torch.Tensor, weight: Weight4) -> torch.Tensor:
-    """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once): the gradient of `linear4`.  Differentiable in A."""
+    """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once; beside 16-bit rows each product is held to 2^-17): the
+    gradient of `linear4`.  Differentiable in A."""
     if type(weight) is Weight4 and torch.is_tensor(A) and _ready(A, weight, weight.n_out, None):
         return _rows(A, weight)
     _check_rows("rows_times_weight4", A, weight, "n_out")

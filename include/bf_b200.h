@@ -723,7 +723,8 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
  *   bf_w4_linear         y [M,n_out] = x [M,n_in] W^T + bias (or NULL); x and y of `type`, sums in fp32.
  *   bf_w4_interval       bounds of the same over boxes, as bf_ibp_linear computes them: W c + b -/+ |W| r; in_mode BF_IN_LOWER_UPPER or
  *                        BF_IN_MID_RAD, relu_in (with BF_IN_LOWER_UPPER) clamps the input at zero first.
- *   bf_w4_rows           z [M,n_in] = a [M,n_out] W: coefficient rows pushed back through the layer, or the gradient of bf_w4_linear.
+ *   bf_w4_rows           z [M,n_in] = a [M,n_out] W: coefficient rows pushed back through the layer, or the gradient of bf_w4_linear (16-bit rows: each
+ *                        product held to 2^-17, sums in fp32).
  *   bf_w4_linear_grad    gradients of x (bf_w4_rows) and of the bias (bf_column_sums) in one call, either NULL where it is not wanted.
  *   bf_w4_interval_grad  gradients of bf_w4_interval (BF_IN_LOWER_UPPER, no relu_in) for those of its two results.
  *   *_many               the same for many rows, on the tensor cores' large tiles, with a workspace of bf_w4_workspace_bytes(M, length of the sum: n_in, or n_out for rows and
