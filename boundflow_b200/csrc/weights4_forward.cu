@@ -1,4 +1,6 @@
 // y = x W^T + bias for few rows x and 4-bit weights, and the bounds of it over boxes (W c -/+ |W| r); weights4_mma.cuh says how.
+#include <math.h>
+
 #include "weights4_mma.cuh"
 
 namespace bf {
@@ -47,10 +49,37 @@ __device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint3
 }
 
 // Digits (P = DIGITS): up to four 16-bit rows as whole numbers of four 8-bit digits, counted in 2^(e - 156) with e the biased exponent of the largest of the row's
-// columns that share a scale (128 of them at most).  A bfloat16 number is held exactly down to 2^-22 of that largest, a half down to 2^-19, and what is smaller within 2^-31 of it.  The codes
+// columns that share a scale (128 of them at most).  A bfloat16 number is held exactly down to 2^-22 of that largest, a half down to 2^-19.  The codes
 // turn into 8-bit numbers, 16 (code - 8), with three operations a word instead of eleven, the integer instruction takes twice as many columns, and its sums are
-// exact; a factor for each column brings them back.  Rows of infinities count those, times infinity; a NaN makes the factor one.
+// exact; a factor for each column brings them back.  What the digits leave of smaller numbers counts where the weights beside the larger ones are zero: where a block meets
+// such a number, `add_rest` multiplies what is left as bfloat16 parts.  Rows of infinities count those, times infinity; a NaN makes the factor one.
 constexpr int DIGITS = 4;
+
+// The exponent that digits are counted from (below 2^-97 the unit stays), by the largest magnitude; the least exponent whose numbers the digits hold whole.
+__device__ __forceinline__ int digits_exponent(float top) { return max((int)(__float_as_uint(top) >> 23), 30); }
+__device__ __forceinline__ int whole_from(int exponent, int type) {
+  return type == BF_TYPE_BF16 ? exponent - 22 : exponent > 132 ? exponent - 19 : 0;  // (halves are multiples of 2^-24)
+}
+__device__ __forceinline__ void eight_numbers(const uint4& q, int type, float (&v)[8]) {
+  const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = type == BF_TYPE_BF16 ? make_float2(__uint_as_float(q4[j] << 16), __uint_as_float(q4[j] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&q4[j]));
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+// Largest magnitude, NaN where one is among them.
+__device__ __forceinline__ float largest_of(const float (&v)[8]) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(v[j]), "f"(v[j + 1]));
+  return top;
+}
+__device__ __forceinline__ float largest_of(float a, float b) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+  return a;
+}
 
 // Parts of the rows' columns [from, to) * 128 in shared memory: [step of 32 columns][product][part, tile][column][4 lanes][8 columns of the step], the 8 in the
 // order 0 4 1 5 2 6 3 7 that `weights_of` gives the codes of a word in (digits: 0 2 4 6 1 3 5 7).  Eight columns of a row are a thread's turn, AHEAD of them are on their way at a time.
@@ -60,6 +89,7 @@ struct Stager {
   Eight<P> raw[AHEAD][SETS];
   int rows[AHEAD], pieces[AHEAD];
   int item, items, piece, row, per_row;
+  bool rest = false;  // digits: some number was not held whole
 
   __device__ __forceinline__ void begin(int from, int to, int M) {
     per_row = (to - from) * (CHUNK / 8);
@@ -86,19 +116,16 @@ struct Stager {
   }
   // Digits of eight columns: their word holds the four, byte by byte (balanced, -128 to 127); a transposition of bytes gives each digit's word of four columns.
   __device__ __forceinline__ void put_digits(const Eight<P>& e, int type, int lanes, int row, int piece, int step_bytes, uint32_t xs, uint32_t factors) {
-    const uint32_t q4[4] = {e.q.x, e.q.y, e.q.z, e.q.w};
     float v[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = type == BF_TYPE_BF16 ? make_float2(__uint_as_float(q4[j] << 16), __uint_as_float(q4[j] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&q4[j]));
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-      top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-    }
+    eight_numbers(e.q, type, v);
+    float top = largest_of(v);
     const uint32_t half = 0xffffu << (threadIdx.x & 16);  // the 16 lanes of a chunk's columns; `lanes` of them share a scale
-    for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(half, top, o));
-    const int exponent = max((int)(top >> 23), 30);  // (below 2^-97 the digits' unit stays)
+    for (int o = lanes >> 1; o > 0; o >>= 1) top = largest_of(top, __shfl_xor_sync(half, top, o));
+    const int exponent = digits_exponent(top);
+    uint32_t least = 0xffffffffu;  // twice the smallest magnitude's bits, less one: zero counts as the largest
+#pragma unroll
+    for (int j = 0; j < 8; ++j) least = min(least, 2u * __float_as_uint(v[j]) - 1u);
+    rest |= exponent < 255 && least < 0xfffffffeu && (int)(least >> 24) < whole_from(exponent, type);
     uint32_t z[8];
     if (exponent < 255) {
       const float scale = __uint_as_float((uint32_t)(283 - exponent) << 23);
@@ -126,7 +153,7 @@ struct Stager {
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         f[d] = ldexpf(1.f, exponent - 160 + 8 * d);
-        if (exponent == 255) f[d] = top > 0x7f800000u ? __int_as_float(0x7fffffff) : d == 0 ? __int_as_float(0x7f800000) : 0.f;
+        if (exponent == 255) f[d] = top != top ? __int_as_float(0x7fffffff) : d == 0 ? __int_as_float(0x7f800000) : 0.f;
       }
       asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(factors + (piece / lanes * NT * 8 + row * 4) * 4), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
     }
@@ -187,6 +214,96 @@ struct Stager {
     }
   }
 };
+
+// What the digits leave of the rows in the warp's chunks: at most 8 bits of a bfloat16 number, 11 of a half, so that one or two bfloat16 parts hold it.  It goes in the column of the
+// row's first digit, on top of the sums of that column, which the warp has laid down at `sums`.  Everything is read again where it lies: this is for the few calls whose numbers lie
+// far apart (in the loop over the chunks the mere branch took one row through 16384 x 16384 from 30 to 34 us).
+template <int NT, int F>
+__device__ __forceinline__ void add_rest(const W4LinearArgs& p, int first, int end, int by, int n0, bool wide, uint32_t sums) {
+  const W4& w = p.w;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long pitch = w.pitch();
+  for (int c = first; c < end; c += by) {
+#pragma unroll 1
+    for (int j = 0; j < NT; ++j) {
+      const int m = 2 * j + (g >> 2);
+      const bool mine = (g & 3) == 0 && m < p.M;
+      Eight<1> raw[4];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const int k = c * CHUNK + step * 32 + t * 8;
+        raw[step].q = make_uint4(0, 0, 0, 0);
+        if (mine) raw[step] = load8<1>(p.a, (long long)m * w.n_in + k, w.n_in - k, wide);
+      }
+      float top[4];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        float v[8];
+        eight_numbers(raw[step].q, p.type, v);
+        top[step] = largest_of(v);
+        top[step] = largest_of(top[step], __shfl_xor_sync(0xffffffffu, top[step], 1));
+        top[step] = largest_of(top[step], __shfl_xor_sync(0xffffffffu, top[step], 2));
+        if (step % F > 0) top[step] = largest_of(top[step], top[step - 1]);  // (complete at a group's last step)
+      }
+      float acc[2][4];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const int exponent = digits_exponent(top[step / F * F + F - 1]), k = c * CHUNK + step * 32 + t * 8;
+        const float unit = __uint_as_float((uint32_t)(exponent - 29) << 23), per_unit = __uint_as_float((uint32_t)(283 - exponent) << 23);
+        float left[8];
+        eight_numbers(raw[step].q, p.type, left);
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          left[i] = exponent < 255 ? left[i] - rintf(left[i] * per_unit) * unit : 0.f;
+          some |= left[i] != 0.f;
+        }
+        if (step % F == 0) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[r][i] = 0.f;
+        }
+        if (__any_sync(0xffffffffu, some)) {
+          uint32_t parts[2][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t q[2];
+            two_numbers_checked<2>(left[i], left[i + 4], q);
+            parts[0][i] = q[0];
+            parts[1][i] = q[1];
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            uint32_t word[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              word[i] = k / 2 < pitch ? *reinterpret_cast<const uint32_t*>(w.codes + (long long)min(n0 + r * 16 + g + 8 * i, w.n_out - 1) * pitch + k / 2) : 0u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a[4] = {weights_of(word[0] >> (8 * h)), weights_of(word[1] >> (8 * h)), weights_of(word[0] >> (8 * h + 4)), weights_of(word[1] >> (8 * h + 4))};
+              mma(acc[r], a[0], a[1], a[2], a[3], parts[0][2 * h], parts[0][2 * h + 1]);
+              mma(acc[r], a[0], a[1], a[2], a[3], parts[1][2 * h], parts[1][2 * h + 1]);
+            }
+          }
+        }
+        if (step % F == F - 1) {
+          const float* scales = w.scales + (long long)min((c * CHUNK + step * 32) >> w.group_log2, w.groups() - 1) * w.n_out;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = r * 16 + g + (i >> 1) * 8;
+              const uint32_t at = sums + ((j * 8 + 2 * t + (i & 1)) * 36 + row) * 4;
+              if (acc[r][i] != 0.f)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(fmaf(scales[min(n0 + row, w.n_out - 1)], acc[r][i], __uint_as_float(lds32(at)))) : "memory");
+            }
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
 
 // P parts of a row, side by side in the columns of NT tiles (PACKED) or an instruction each for NT tiles of 8 rows; DUAL: W c and |W| r; F: steps of 32 columns
 // that share a scale (1, 2, or 4 and more).
@@ -381,6 +498,9 @@ __global__ void __launch_bounds__(THREADS, (PACKED ? 1 : P) * NT * (DUAL ? 2 : 1
         for (int i = 0; i < 4; ++i)
           asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (((s * NT + j) * 8 + 2 * t + (i & 1)) * 36 + r * 16 + g + (i >> 1) * 8) * 4), "f"(tot[s][r][j][i]) : "memory");
   __syncwarp();
+  if constexpr (P == DIGITS) {
+    if (__syncthreads_or(stager.rest)) add_rest<NT, F>(p, first + kw, end, sp.kw, n0, wide, ring);
+  }
   if (sp.cluster > 1) cluster_wait();
   {
     const int owner = lane >> each_log2;
