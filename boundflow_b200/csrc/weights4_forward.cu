@@ -52,7 +52,7 @@ __device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint3
 // columns that share a scale (128 of them at most).  A bfloat16 number is held exactly down to 2^-22 of that largest, a half down to 2^-19.  The codes
 // turn into 8-bit numbers, 16 (code - 8), with three operations a word instead of eleven, the integer instruction takes twice as many columns, and its sums are
 // exact; a factor for each column brings them back.  What the digits leave of smaller numbers counts where the weights beside the larger ones are zero: where a block meets
-// such a number, `add_rest` multiplies what is left as bfloat16 parts.  Rows of infinities count those, times infinity; a NaN makes the factor one.
+// such a number, `add_rest` multiplies what is left as bfloat16 parts, and infinities and NaN, of which the digits hold nothing: each meets its own weight.
 constexpr int DIGITS = 4;
 
 // The exponent that digits are counted from (below 2^-97 the unit stays), by the largest magnitude; the least exponent whose numbers the digits hold whole.
@@ -75,6 +75,10 @@ __device__ __forceinline__ float largest_of(const float (&v)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(v[j]), "f"(v[j + 1]));
   return top;
+}
+__device__ __forceinline__ void finite_only(float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) < INFINITY ? v[j] : 0.f;
 }
 __device__ __forceinline__ float largest_of(float a, float b) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
@@ -121,20 +125,22 @@ struct Stager {
     float top = largest_of(v);
     const uint32_t half = 0xffffu << (threadIdx.x & 16);  // the 16 lanes of a chunk's columns; `lanes` of them share a scale
     for (int o = lanes >> 1; o > 0; o >>= 1) top = largest_of(top, __shfl_xor_sync(half, top, o));
+    if (!(top < INFINITY)) {  // (the lanes that share a scale come here together)
+      rest = true;
+      finite_only(v);
+      top = largest_of(v);
+      const uint32_t group = ((1u << lanes) - 1u) << (threadIdx.x & 31 & -lanes);
+      for (int o = lanes >> 1; o > 0; o >>= 1) top = largest_of(top, __shfl_xor_sync(group, top, o));
+    }
     const int exponent = digits_exponent(top);
     uint32_t least = 0xffffffffu;  // twice the smallest magnitude's bits, less one: zero counts as the largest
 #pragma unroll
     for (int j = 0; j < 8; ++j) least = min(least, 2u * __float_as_uint(v[j]) - 1u);
-    rest |= exponent < 255 && least < 0xfffffffeu && (int)(least >> 24) < whole_from(exponent, type);
+    rest |= least < 0xfffffffeu && (int)(least >> 24) < whole_from(exponent, type);
     uint32_t z[8];
-    if (exponent < 255) {
-      const float scale = __uint_as_float((uint32_t)(283 - exponent) << 23);
+    const float scale = __uint_as_float((uint32_t)(283 - exponent) << 23);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] = ((uint32_t)__float2int_rn(v[j] * scale) + 0x00808080u) ^ 0x00808080u;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] = isinf(v[j]) ? (v[j] > 0.f ? 0x00000001u : 0x000000ffu) : 0u;
-    }
+    for (int j = 0; j < 8; ++j) z[j] = ((uint32_t)__float2int_rn(v[j] * scale) + 0x00808080u) ^ 0x00808080u;
     const uint32_t to = xs + (piece >> 2) * step_bytes + (row * 4 * 4 + (piece & 3)) * 8;
     uint32_t o[2][4];
 #pragma unroll
@@ -151,10 +157,7 @@ struct Stager {
     if ((piece & (lanes - 1)) == 0) {  // 2^(e - 156) / 16 and the digits' places
       float f[4];
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        f[d] = ldexpf(1.f, exponent - 160 + 8 * d);
-        if (exponent == 255) f[d] = top != top ? __int_as_float(0x7fffffff) : d == 0 ? __int_as_float(0x7f800000) : 0.f;
-      }
+      for (int d = 0; d < 4; ++d) f[d] = ldexpf(1.f, exponent - 160 + 8 * d);
       asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(factors + (piece / lanes * NT * 8 + row * 4) * 4), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
     }
   }
@@ -240,6 +243,7 @@ __device__ __forceinline__ void add_rest(const W4LinearArgs& p, int first, int e
       for (int step = 0; step < 4; ++step) {
         float v[8];
         eight_numbers(raw[step].q, p.type, v);
+        finite_only(v);
         top[step] = largest_of(v);
         top[step] = largest_of(top[step], __shfl_xor_sync(0xffffffffu, top[step], 1));
         top[step] = largest_of(top[step], __shfl_xor_sync(0xffffffffu, top[step], 2));
@@ -255,7 +259,7 @@ __device__ __forceinline__ void add_rest(const W4LinearArgs& p, int first, int e
         bool some = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          left[i] = exponent < 255 ? left[i] - rintf(left[i] * per_unit) * unit : 0.f;
+          if (fabsf(left[i]) < INFINITY) left[i] -= rintf(left[i] * per_unit) * unit;
           some |= left[i] != 0.f;
         }
         if (step % F == 0) {

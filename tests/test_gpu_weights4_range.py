@@ -83,3 +83,28 @@ def test_all_magnitudes_and_many_zero_weights(dev, kind, group):
         got = linear4(x, W)
         check(got, x, w)
         assert torch.equal(linear4(x[:1], W), got[:1]) or m == 5  # the same bits alone and beside other rows
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,k,group", [(60, 200, 32), (60, 200, 64), (61, 300, 128), (60, 700, 512)])
+def test_several_infinities_in_a_group(dev, kind, n, k, group):
+    """Infinity times zero is NaN and so are infinities of both signs in one sum, whatever else the group holds; the rows beside are as they are without."""
+    from boundflow_b200.weights4 import linear4
+
+    W, w, g = weight(n, k, group, dev, [3, 9])
+    places = [{1: "inf", 2: "inf"}, {1: "inf", 2: "-inf"}, {3: "inf", 4: "inf"}, {3: "-inf", 9: "inf", k - 1: "inf"}, {5: "inf", 6: "nan"}, {c: "inf" for c in range(k)},
+              {c: "-inf" for c in range(20, 31)}, {40: "inf"}]
+    for m in (1, 2, 3, 4, 5):
+        x = torch.randn(m, k, generator=g).to(TYPES[kind]).to(dev)
+        clean = linear4(x, W)
+        for row in range(m):
+            for place in places:
+                y = x.clone()
+                for c, v in place.items():
+                    y[row, c] = float(v)
+                got, want = linear4(y, W), (y.double().cpu() @ w.t().cpu()).to(dev)
+                assert torch.equal(got[row].isnan(), want[row].isnan()), (m, row, place)
+                inf = want[row].isinf()
+                assert torch.equal(got[row][inf].double(), want[row][inf]) and bool((got[row].isnan() | got[row].isinf()).all())
+                others = [i for i in range(m) if i != row]
+                assert torch.equal(got[others], clean[others])
