@@ -9,8 +9,9 @@
 //     columns that share a scale (at most 128 of them) is taken on the tensor cores, into one of two accumulators; from there the eight warps add it, times the scale,
 //     to sums in their registers while the other is filled.
 //   a W: the scale belongs to the summed index, so it goes into the weight: scale * (code - 8) as a sum of two bfloat16 numbers (16-bit rows: off by 2^-17 and, the scale being
-//     held in two parts then, 2^-18), or three (fp32 rows), rounded to the nearest each, and products of parts below 2^-17 (2^-26) of the whole are left out.  All sums stay on the tensor cores.  Weights of two parts would
-//     make NaN of a row's infinity, so numbers that are not finite are left out of the images and their rows are summed by plain arithmetic at the end.
+//     held in two parts then, 2^-18), or three (fp32 rows), rounded to the nearest each, and products of parts below 2^-17 (2^-26) of the whole are left out.  All sums stay on the tensor cores.  A weight's
+//     second part would make NaN of a row's infinity, so where a stage's image holds numbers that are not finite (a bit says so) the image as it is meets the weights' first parts, and a
+//     copy that the copying warp clears of them in shared memory meets the others.
 //
 // Waits are bounded: where one runs out, the block raises the status word, frees its tensor memory and stores NaN.
 //
@@ -37,16 +38,17 @@ constexpr int A_BYTES = LANES * STEP * 2;
 // Warps: eight that sum, pairs that unpack a stage each in turn, one that copies, one that issues.  Launched with 128 registers a thread; the eight take 168 (they hold up
 // to 128 sums), for which the others give up all but 80: 256 * 168 + 256 * 80 is within 512 * 128.
 constexpr int SUMMERS = 8, TEAM = 64, COPIER = 14, ISSUER = 15, THREADS = 512;
-constexpr int HEADER = 1024;          // of the workspace: the status word, then a byte for each row that is not finite
+constexpr int HEADER = 1024;          // of the workspace: the status word, then a bit for each tile of rows and 64 summed indices that hold a number that is not finite
 constexpr int RING = 224 * 1024;
 
 enum { TAKE_ROWS = 0, TAKE_CENTRE = 1, TAKE_RADIUS = 2, TAKE_SUM = 3, TAKE_DIFFERENCE = 4 };
+__host__ __device__ constexpr int words_of(int steps) { return (steps + 31) / 32; }  // of the bits of a tile of rows
 
 struct ManyArgs {
   W4 w;
   const uint8_t* images;
-  const uint8_t* odd;   // a W: rows that hold an infinity or a NaN
-  const void* a;        // the rows themselves, for those
+  const uint32_t* odd;  // a W: bits [row tile][step]
+  const void* a;
   const float* b;
   const void* bias;
   void* out;
@@ -56,7 +58,7 @@ struct ManyArgs {
 };
 
 struct Control {
-  unsigned long long a_full[4], a_empty[4], b_full[8], b_empty[8], d_full[2], d_empty[2];
+  unsigned long long a_full[4], a_empty[4], b_full[8], b_empty[8], d_full[2], d_empty[2], copied;
   uint32_t tmem;
   int abort_flag;
 };
@@ -108,19 +110,12 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t w) {
 }
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
-// The number that a product takes for element `at` of the rows.
-__device__ __forceinline__ float taken(const void* a, const float* b, int type, int take, long long at) {
-  if (take == TAKE_ROWS) return load_any(a, type, at);
-  const float x = static_cast<const float*>(a)[at], y = b[at];
-  return take == TAKE_CENTRE ? 0.5f * (x + y) : take == TAKE_RADIUS ? 0.5f * (y - x) : take == TAKE_SUM ? x + y : y - x;
-}
-
 // ---- images of the rows ----------------------------------------------------------------
 struct ImageArgs {
   const void* a;
   const float* b;
   uint8_t* images;
-  uint8_t* odd;
+  uint32_t* odd;
   int* status;
   int type, take, mode, relu_in, M, n, tile_m, steps;
 };
@@ -187,14 +182,16 @@ __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) 
       }
     }
     uint32_t out[PARTS][4];
-    bool strange = false;
+    bool strange = false, infinite = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      bool fits = fabsf(v[j]) < 3.3e38f;  // (above that a number rounds to infinity)
-      if (PARTS == 1) fits = FORWARD || fabsf(v[j]) < INFINITY;
-      if (fits) continue;
-      if (FORWARD) strange = true;
-      else { p.odd[m] = 1; v[j] = 0.f; }
+      strange |= !(fabsf(v[j]) < 3.3e38f);  // (above that a number rounds to infinity)
+      infinite |= !(fabsf(v[j]) < INFINITY);
+    }
+    if (!FORWARD && infinite) {
+      uint32_t* word = p.odd + (long long)((unsigned)m >> (31 - __clz(p.tile_m))) * words_of(p.steps) + (eight >> 8);
+      const uint32_t bit = 1u << ((eight >> 3) & 31);
+      if ((*reinterpret_cast<volatile uint32_t*>(word) & bit) == 0) atomicOr(word, bit);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -212,7 +209,7 @@ __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) 
         }
       }
     }
-    if (FORWARD && PARTS > 1 && strange) {  // infinities and NaN are one part; the largest numbers are cut to theirs
+    if (PARTS > 1 && strange) {  // infinities and NaN are one part; the largest numbers are cut to theirs
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (fabsf(v[j]) < 3.3e38f) continue;
@@ -224,7 +221,7 @@ __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) 
           part[1] = (uint16_t)(__float_as_uint(rest) >> 16);
           part[2] = (uint16_t)(__float_as_uint(rest - __uint_as_float(__float_as_uint(rest) & 0xffff0000u)) >> 16);
         }
-        const int word = j & 3, high = j >> 2;
+        const int word = FORWARD ? j & 3 : j >> 1, high = FORWARD ? j >> 2 : j & 1;
 #pragma unroll
         for (int k = 0; k < PARTS; ++k) {
           const uint32_t keep = high ? 0x0000ffffu : 0xffff0000u;
@@ -274,6 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
       mbar_init(smem_u32(&ctl->b_full[s]), 1);
       mbar_init(smem_u32(&ctl->b_empty[s]), 1);
     }
+    mbar_init(smem_u32(&ctl->copied), 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&ctl->d_full[s]), 1);
       mbar_init(smem_u32(&ctl->d_empty[s]), SUMMERS);
@@ -293,20 +291,71 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
   const int units = FORWARD ? (UNIT == 1 ? 2 * H : UNIT == 2 ? H : (H + 1) / 2) : 1;
 
   const uint8_t* images = p.images + (long long)blockIdx.y * H * XP * B_BYTES;
+  const uint32_t* odd = p.odd + (long long)blockIdx.y * words_of(H);
   if (warp >= SUMMERS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == COPIER) {
-      if (elected()) {
-        const int items = H * XP;
-        int asked = 0;
-        for (; asked < items; ++asked) {
-          const int s = asked % BS;
-          if (asked >= BS && !mbar_wait(smem_u32(&ctl->b_empty[s]), (uint32_t)(asked / BS - 1) & 1u, abort_flag)) break;
-          mbar_arrive_expect_tx(smem_u32(&ctl->b_full[s]), B_BYTES);
-          bulk_copy_g2s(b_ring + s * B_BYTES, images + (long long)asked * B_BYTES, B_BYTES, smem_u32(&ctl->b_full[s]));
+      // The numbers of a stage's image that are not finite, with zeros in their place: what the weights' later parts are multiplied by.
+      auto clear = [&](uint32_t at) {
+        for (int i = lane * 16; i < B_BYTES; i += 512) {
+          uint32_t v[4];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at + i) : "memory");
+          bool some = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t keep = ((v[j] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((v[j] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+            some |= keep != 0xffffffffu;
+            v[j] &= keep;
+          }
+          if (some) put16(at + i, v);
         }
-        if (asked < items) drain_bulk_copies(ctl->b_full, BS, asked);  // copies in flight land before the block ends
+      };
+      const bool one = elected();
+      bool ok = true;  // (of the one)
+      int asked = 0;
+      uint32_t copied_phase = 0, bits = 0;
+      for (int h = 0; h < H; ++h) {
+        if (!FORWARD && (h & 31) == 0) bits = __ldg(odd + (h >> 5));
+        const bool infinite = !FORWARD && ((bits >> (h & 31)) & 1u) != 0;
+        for (int part = 0; part < XP; ++part) {
+          const uint8_t* image = images + ((long long)h * XP + part) * B_BYTES;
+          if (one && ok) {
+            const int s = asked % BS;
+            ok = asked < BS || mbar_wait(smem_u32(&ctl->b_empty[s]), (uint32_t)(asked / BS - 1) & 1u, abort_flag);
+            if (ok) {
+              mbar_arrive_expect_tx(smem_u32(&ctl->b_full[s]), B_BYTES);
+              bulk_copy_g2s(b_ring + s * B_BYTES, image, B_BYTES, smem_u32(&ctl->b_full[s]));
+              ++asked;
+            }
+          }
+          if (part == 0 && infinite) {
+            int at = -1;
+            if (one && ok) {
+              const int s = asked % BS;
+              ok = asked < BS || mbar_wait(smem_u32(&ctl->b_empty[s]), (uint32_t)(asked / BS - 1) & 1u, abort_flag);
+              if (ok) {
+                mbar_arrive_expect_tx(smem_u32(&ctl->copied), B_BYTES);
+                bulk_copy_g2s(b_ring + s * B_BYTES, image, B_BYTES, smem_u32(&ctl->copied));
+                at = s;
+              }
+            }
+            at = __reduce_max_sync(0xffffffffu, at);
+            if (at < 0) continue;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->copied), copied_phase, abort_flag))) {
+              if (one) drain_bulk_copies(&ctl->copied, 1, (int)copied_phase + 1);
+              ok = false;
+              continue;
+            }
+            copied_phase ^= 1u;
+            clear(b_ring + at * B_BYTES);
+            fence_proxy_async();
+            __syncwarp();
+            if (one) mbar_arrive(smem_u32(&ctl->b_full[at]));
+            ++asked;
+          }
+        }
       }
+      if (one && !ok) drain_bulk_copies(ctl->b_full, BS, asked);  // copies in flight land before the block ends
       __syncwarp();
     } else if (warp == ISSUER) {
       if (elected()) {
@@ -323,7 +372,12 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
         auto unit_begins = [&]() {
           if (FORWARD && unit >= 2) wait(ctl->d_empty[unit & 1], (uint32_t)(unit / 2 - 1) & 1u);
         };
+        uint32_t bits = FORWARD ? 0u : __ldg(odd), next_bits = FORWARD ? 0u : __ldg(odd + min(1, words_of(H) - 1));
         for (int h = 0; ok && h < H; ++h) {
+          if (!FORWARD && h > 0 && (h & 31) == 0) {
+            bits = next_bits;
+            next_bits = __ldg(odd + min((h >> 5) + 1, words_of(H) - 1));
+          }
           wait(ctl->a_full[as], a_phase);
           const uint64_t a = a_first + (uint64_t)(as * WP * (A_BYTES >> 4));
           if (FORWARD && UNIT == 1) {  // two units a stage
@@ -357,10 +411,20 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
               wait(ctl->b_full[slot], b_phase);
               tc_fence_after();
               if (!ok) break;
-              const uint64_t b = b_first + (uint64_t)(slot * (B_BYTES >> 4));
+              uint64_t b = b_first + (uint64_t)(slot * (B_BYTES >> 4));
 #pragma unroll
-              for (int q = 0; q < WP; ++q)
+              for (int q = 0; q < WP; ++q) {
+                if (!FORWARD && part == 0 && q == 1 && ((bits >> (h & 31)) & 1u) != 0) {  // from here on without what is not finite
+                  mma_commit(smem_u32(&ctl->b_empty[slot]));
+                  if (++slot == BS) { slot = 0; b_phase ^= 1u; }
+                  wait(ctl->b_full[slot], b_phase);
+                  tc_fence_after();
+                  if (!ok) break;
+                  b = b_first + (uint64_t)(slot * (B_BYTES >> 4));
+                }
                 if (FORWARD || q + part < WP) mma_step<SLICE>(d, a + (uint64_t)(q * (A_BYTES >> 4)), b, idesc, !(anew && part == 0 && q == 0));
+              }
+              if (!ok) break;
               mma_commit(smem_u32(&ctl->b_empty[slot]));
               if (++slot == BS) { slot = 0; b_phase ^= 1u; }
             }
@@ -515,22 +579,11 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
     const float bias = FORWARD && p.bias && !absolute && of < width ? load_any(p.bias, p.bias_type, of) : 0.f;
     if (of < width) {
       const int m1 = m0 + (warp >> 2) * CW;
-      auto finish = [&](int m, float v) {
-        const long long at = (long long)m * width + of;
-        if (absolute) {
-          float* out = static_cast<float*>(p.out);
-          const float c = out[at];
-          out[at] = FORWARD ? c - v : 0.5f * (c - v);
-          p.out2[at] = FORWARD ? c + v : 0.5f * (c + v);
-        } else {
-          store_any(p.out, p.type, at, v);
-        }
-      };
       const long long first = (long long)m1 * width + of;
       auto rows = [&](auto* out, auto round) {
 #pragma unroll
         for (int j = 0; j < CW; ++j)
-          if (m1 + j < p.M && (FORWARD || p.odd[m1 + j] == 0)) out[first + (long long)j * width] = round(acc[j]);
+          if (m1 + j < p.M) out[first + (long long)j * width] = round(acc[j]);
       };
 #pragma unroll
       for (int j = 0; j < CW; ++j) acc[j] = alive ? acc[j] + bias : __int_as_float(0x7fffffff);
@@ -544,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
           for (int j = 0; j < BATCH; ++j) c[j] = m1 + j0 + j < p.M ? out[(long long)(j0 + j) * width] : 0.f;
 #pragma unroll
           for (int j = 0; j < BATCH; ++j) {
-            if (m1 + j0 + j >= p.M || (!FORWARD && p.odd[m1 + j0 + j] != 0)) continue;
+            if (m1 + j0 + j >= p.M) continue;
             const float v = acc[j0 + j];
             out[(long long)(j0 + j) * width] = FORWARD ? c[j] - v : 0.5f * (c[j] - v);
             p.out2[first + (long long)(j0 + j) * width] = FORWARD ? c[j] + v : 0.5f * (c[j] + v);
@@ -556,18 +609,6 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
         rows(static_cast<__nv_bfloat16*>(p.out), [](float v) { return __float2bfloat16(v); });
       } else {
         rows(static_cast<__half*>(p.out), [](float v) { return __float2half(v); });
-      }
-      if (!FORWARD) {  // rows that the products could not take
-        for (int m = m1; m < min(m1 + CW, p.M); ++m) {
-          if (p.odd[m] == 0) continue;
-          float v = 0.f;
-          for (int n = 0; n < w.n_out; ++n) {
-            const uint32_t byte = w.codes[n * pitch + of / 2];
-            const float weight = w.scales[(long long)(of >> w.group_log2) * w.n_out + n] * (float)((int)((byte >> (4 * (of & 1))) & 15u) - 8);
-            v = fmaf(taken(p.a, p.b, p.type, p.take, (long long)m * w.n_out + n), absolute ? fabsf(weight) : weight, v);
-          }
-          finish(m, v);
-        }
       }
     }
     if (!alive && lane == 0) *p.status = 1;
@@ -586,8 +627,9 @@ int rows_of_block(int M, int features) {
   if (M > 128 && tiles * ceil_div(M, 256) >= 148) return 256;
   return M > 64 ? 128 : 64;
 }
-size_t header_of(int M) { return HEADER + (size_t)ceil_div(M, 1024) * 1024; }
 int steps_of(int n) { return ceil_div(n, STEP); }
+size_t odd_bytes(int M, int sum) { return (size_t)ceil_div(M, 64) * words_of(steps_of(sum)) * 4; }  // (the smallest tiles)
+size_t header_of(int M, int sum) { return HEADER + (odd_bytes(M, sum) + 1023) / 1024 * 1024; }
 int parts_of(int type) { return type == BF_TYPE_F32 ? 3 : type == BF_TYPE_F16 ? 2 : 1; }
 
 template <int XP, int WP, int CW, int UNIT>
@@ -632,11 +674,12 @@ int pass(const ManyArgs& all, int mode, int relu_in, void* workspace, bool first
     p.out2 = all.out2 ? all.out2 + done * features : nullptr;
     p.steps = steps_of(sum);
     p.status = reinterpret_cast<int*>(base);
-    p.odd = base + HEADER;
-    p.images = base + header_of(slab);
+    uint32_t* odd = reinterpret_cast<uint32_t*>(base + HEADER);
+    p.odd = odd;
+    p.images = base + header_of(slab, sum);
     const int tile_m = rows_of_block(p.M, features);
-    const ImageArgs im = {p.a, p.b, base + header_of(slab), base + HEADER, first_pass && done == 0 ? p.status : nullptr, p.type, p.take, mode, relu_in, p.M, sum, tile_m, p.steps};
-    if (!FORWARD && cudaMemsetAsync(base + HEADER, 0, p.M, stream) != cudaSuccess) {
+    const ImageArgs im = {p.a, p.b, base + header_of(slab, sum), odd, first_pass && done == 0 ? p.status : nullptr, p.type, p.take, mode, relu_in, p.M, sum, tile_m, p.steps};
+    if (!FORWARD && cudaMemsetAsync(odd, 0, odd_bytes(p.M, sum), stream) != cudaSuccess) {
       set_error("w4_rows_images_kernel: cannot clear the workspace");
       return BF_E_CUDA;
     }
@@ -674,7 +717,7 @@ bool w4_many_pays(int M, int n_in, int n_out, int group, int type, bool forward,
 
 long long w4_many_bytes(int M, int sum, int type) {
   const int slab = slab_of(M, sum, type);
-  return (long long)header_of(slab) + (long long)ceil_div(slab, 256) * 256 * steps_of(sum) * 128 * parts_of(type);  // enough for blocks of any size
+  return (long long)header_of(slab, sum) + (long long)ceil_div(slab, 256) * 256 * steps_of(sum) * 128 * parts_of(type);  // enough for blocks of any size
 }
 int launch_w4_linear_many(const W4LinearArgs& l, void* workspace, cudaStream_t stream) {
   ManyArgs p = {};
