@@ -9,7 +9,9 @@
 //     columns that share a scale (at most 128 of them) is taken on the tensor cores, into one of two accumulators; from there the eight warps add it, times the scale,
 //     to sums in their registers while the other is filled.
 //   a W: the scale belongs to the summed index, so it goes into the weight: scale * (code - 8) as a sum of two bfloat16 numbers (16-bit rows: off by 2^-17 and, the scale being
-//     held in two parts then, 2^-18), or three (fp32 rows), rounded to the nearest each, and products of parts below 2^-17 (2^-26) of the whole are left out.  All sums stay on the tensor cores.  A weight's
+//     held in two parts then, 2^-18), or three (fp32 rows), rounded to the nearest each, and products of parts below 2^-17 (2^-26) of the whole are left out.  Tensor-memory accumulators truncate, by half a unit in the last
+//     place of the running sum for every 16 terms of a product and always in the same direction, so a sum ends after `back_stages` and is added to the registers in the same way
+//     (fp32 rows of 1024 to 65536 terms against 64 bits, 2-norm: 1.1e-6 to 1.2e-6; 8192 terms in one sum 5.3e-5, the FP32 kernel on the dense weight 5e-7 to 4e-6).  A weight's
 //     second part would make NaN of a row's infinity, so where a stage's image holds numbers that are not finite (a bit says so) the image as it is meets the weights' first parts, and a
 //     copy that the copying warp clears of them in shared memory meets the others.
 //
@@ -38,6 +40,7 @@ constexpr int A_BYTES = LANES * STEP * 2;
 // Warps: eight that sum, pairs that unpack a stage each in turn, one that copies, one that issues.  Launched with 128 registers a thread; the eight take 168 (they hold up
 // to 128 sums), for which the others give up all but 80: 256 * 168 + 256 * 80 is within 512 * 128.
 constexpr int SUMMERS = 8, TEAM = 64, COPIER = 14, ISSUER = 15, THREADS = 512;
+__host__ __device__ constexpr int back_stages(int weight_parts) { return weight_parts == 3 ? 2 : 8; }  // of a sum of a W: 48 MMA steps (six products of parts), or 64 to 96 beside a result of 16 bits
 constexpr int HEADER = 1024;          // of the workspace: the status word, then a bit for each tile of rows and 64 summed indices that hold a number that is not finite
 constexpr int RING = 224 * 1024;
 
@@ -288,7 +291,8 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const int units = FORWARD ? (UNIT == 1 ? 2 * H : UNIT == 2 ? H : (H + 1) / 2) : 1;
+  constexpr int SPAN = !FORWARD ? back_stages(WP) : UNIT >= 4 ? 2 : 1;  // stages of a sum (x W^T with scales for 32 columns: half a stage)
+  const int units = FORWARD && UNIT == 1 ? 2 * H : (H + SPAN - 1) / SPAN;
 
   const uint8_t* images = p.images + (long long)blockIdx.y * H * XP * B_BYTES;
   const uint32_t* odd = p.odd + (long long)blockIdx.y * words_of(H);
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
         bool ok = true;
         auto wait = [&](unsigned long long& bar, uint32_t phase) { return ok = ok && mbar_wait(smem_u32(&bar), phase, abort_flag); };
         auto unit_begins = [&]() {
-          if (FORWARD && unit >= 2) wait(ctl->d_empty[unit & 1], (uint32_t)(unit / 2 - 1) & 1u);
+          if (unit >= 2) wait(ctl->d_empty[unit & 1], (uint32_t)(unit / 2 - 1) & 1u);
         };
         uint32_t bits = FORWARD ? 0u : __ldg(odd), next_bits = FORWARD ? 0u : __ldg(odd + min(1, words_of(H) - 1));
         for (int h = 0; ok && h < H; ++h) {
@@ -404,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
               ++unit;
             }
           } else {
-            const bool anew = FORWARD ? (UNIT == 2 || h % 2 == 0) : h == 0;
+            const bool anew = h % SPAN == 0;
             if (anew) unit_begins();
             const uint32_t d = tmem + (unit & 1) * TM;
             for (int part = 0; part < XP; ++part) {
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
             }
             if (!ok) break;
             mma_commit(smem_u32(&ctl->a_empty[as]));
-            if (h == H - 1 || (FORWARD && (UNIT == 2 || h % 2 == 1))) {
+            if (h == H - 1 || h % SPAN == SPAN - 1) {
               mma_commit(smem_u32(&ctl->d_full[unit & 1]));
               ++unit;
             }
@@ -546,8 +550,8 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
       const int buffer = u & 1;
       const float s = next_scale;
       if (FORWARD && u + 1 < units) next_scale = unit_scale(u + 1);
-      if (!FORWARD)  // (all the products long: asleep, they leave the others the issue slots)
-        for (int i = 0; i < 4000000 && !mbar_try_wait(smem_u32(&ctl->d_full[0]), 0) && *abort_flag == 0; ++i) __nanosleep(500);
+      if (!FORWARD)  // (they wait for long: asleep, they leave the others the issue slots)
+        for (int i = 0; i < 4000000 && !mbar_try_wait(smem_u32(&ctl->d_full[buffer]), (uint32_t)(u / 2) & 1u) && *abort_flag == 0; ++i) __nanosleep(500);
       if (!mbar_wait_warp(smem_u32(&ctl->d_full[buffer]), (uint32_t)(u / 2) & 1u, abort_flag)) { alive = false; break; }
       tc_fence_after();
 #pragma unroll
@@ -564,8 +568,8 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
                 : "+f"(acc[c + j]), "+f"(acc[c + j + 1])
                 : "f"(v[j]), "f"(v[j + 1]), "f"(s));
           } else {
-            acc[c + j] = v[j];
-            acc[c + j + 1] = v[j + 1];
+            acc[c + j] += v[j];
+            acc[c + j + 1] += v[j + 1];
           }
         }
       }
