@@ -12,8 +12,13 @@ namespace {
 // row or two the tensor cores are 41% and the issue slots 49% busy with 16 warps an SM; with one row the parts, which each warp makes for every 32 outputs, and four
 // loads of shared memory for 1024 codes bound it.
 //
+// The matrix instruction truncates what it adds to, always in the same direction: sums that stay in it over 192 instructions are off by 7e-6 where all terms are positive.  Three and more fp32 rows
+// end them after at most MOST_IN_ONE outputs times 32, by more blocks or (SHORT) by an addition in 32 bits after every 32 outputs; `backward` chooses.  (16-bit rows do not: their results
+// are rounded to 2^-9 or 2^-12.)
+//
 // P parts of a row, side by side (PACKED, one tile) or an instruction each for NT tiles of 8 rows; STEPS of 32 columns share a scale (1, 2, or 4 and more).
-template <int P, bool PACKED, int NT, bool DUAL, int STEPS>
+constexpr int MOST_IN_ONE = 8;
+template <int P, bool PACKED, int NT, bool DUAL, int STEPS, bool SHORT>
 __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p, const Split sp) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int Q = PACKED ? 1 : P * NT, SETS = DUAL ? 2 : 1;
@@ -147,9 +152,7 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
         }
         __syncwarp();
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t b[SETS][Q][2];
+      auto load_b = [&](int h, uint32_t (&b)[SETS][Q][2]) {
 #pragma unroll
         for (int s = 0; s < SETS; ++s)
 #pragma unroll
@@ -158,23 +161,79 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
                          : "=r"(b[s][q][0]), "=r"(b[s][q][1])
                          : "r"(as + s * set_bytes + ((q * cv + min(g, cv - 1)) * 32 + h * 16 + 4 * t) * 2)
                          : "memory");
+      };
+      // Codes of 32 columns and 16 outputs: lo, hi as the instruction takes them.
+      auto load_codes_of = [&](int h, int step, uint32_t& lo, uint32_t& hi) {
+        const uint32_t row = st + (h * 16 + 2 * t) * ROW_BYTES + (step * 4 + (g & 3)) * 4;
+        const uint32_t w0 = lds32(row), w1 = lds32(row + ROW_BYTES), w8 = lds32(row + 8 * ROW_BYTES), w9 = lds32(row + 9 * ROW_BYTES);
+        const uint32_t sel = g >= 4 ? 0x7632u : 0x5410u;
+        lo = __byte_perm(w0, w1, sel);
+        hi = __byte_perm(w8, w9, sel);
+      };
+      auto weights = [&](uint32_t lo, uint32_t hi, int e, uint32_t (&a)[4]) {
+        a[0] = weights_of(lo >> (8 * e));
+        a[1] = weights_of(lo >> (8 * e + 4));
+        a[2] = weights_of(hi >> (8 * e));
+        a[3] = weights_of(hi >> (8 * e + 4));
+      };
+      if constexpr (SHORT) {
+        uint32_t b[2][SETS][Q][2];
+        load_b(0, b[0]);
+        load_b(1, b[1]);
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
           const int step = group * STEPS + i;
-          const uint32_t row = st + (h * 16 + 2 * t) * ROW_BYTES + (step * 4 + (g & 3)) * 4;
-          const uint32_t w0 = lds32(row), w1 = lds32(row + ROW_BYTES), w8 = lds32(row + 8 * ROW_BYTES), w9 = lds32(row + 9 * ROW_BYTES);
-          const uint32_t sel = g >= 4 ? 0x7632u : 0x5410u;
-          const uint32_t lo = __byte_perm(w0, w1, sel), hi = __byte_perm(w8, w9, sel);
+          uint32_t lo[2], hi[2];
+          load_codes_of(0, step, lo[0], hi[0]);
+          load_codes_of(1, step, lo[1], hi[1]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t a[4] = {weights_of(lo >> (8 * e)), weights_of(lo >> (8 * e + 4)), weights_of(hi >> (8 * e)), weights_of(hi >> (8 * e + 4))};
 #pragma unroll
-            for (int q = 0; q < Q; ++q) mma(acc[0][step][e][q % NT], a[0], a[1], a[2], a[3], b[0][q][0], b[0][q][1]);
-            if (DUAL) {
+            for (int s = 0; s < SETS; ++s) {
+              float sum[NT][4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) a[k] &= 0x7fff7fffu;
+              for (int h = 0; h < 2; ++h) {
+                uint32_t a[4];
+                weights(lo[h], hi[h], e, a);
+                if (s == 1) {
 #pragma unroll
-              for (int q = 0; q < Q; ++q) mma(acc[SETS - 1][step][e][q % NT], a[0], a[1], a[2], a[3], b[SETS - 1][q][0], b[SETS - 1][q][1]);
+                  for (int k = 0; k < 4; ++k) a[k] &= 0x7fff7fffu;
+                }
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                  if (h == 0 && q < NT) mma_anew(sum[q % NT], a[0], a[1], a[2], a[3], b[h][s][q][0], b[h][s][q][1]);
+                  else mma(sum[q % NT], a[0], a[1], a[2], a[3], b[h][s][q][0], b[h][s][q][1]);
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[s][step][e][j][k] += sum[j][k];
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t b[SETS][Q][2];
+          load_b(h, b);
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            const int step = group * STEPS + i;
+            uint32_t lo, hi;
+            load_codes_of(h, step, lo, hi);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t a[4];
+              weights(lo, hi, e, a);
+#pragma unroll
+              for (int q = 0; q < Q; ++q) mma(acc[0][step][e][q % NT], a[0], a[1], a[2], a[3], b[0][q][0], b[0][q][1]);
+              if (DUAL) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) a[k] &= 0x7fff7fffu;
+#pragma unroll
+                for (int q = 0; q < Q; ++q) mma(acc[SETS - 1][step][e][q % NT], a[0], a[1], a[2], a[3], b[SETS - 1][q][0], b[SETS - 1][q][1]);
+              }
             }
           }
         }
@@ -245,21 +304,38 @@ __global__ void __launch_bounds__(THREADS, 2) w4_rows_kernel(const W4RowsArgs p,
   }
 }
 
+template <int P, bool PACKED, int NT, bool DUAL, bool SHORT>
+int launch_groups(const W4RowsArgs& p, const Split& sp, long long blocks, int tiles_m, int smem, cudaStream_t stream) {
+  static SmemOptIn table[3];
+  if (p.w.group_log2 == 5) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 1, SHORT>, "w4_rows_kernel", table[0], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  if (p.w.group_log2 == 6) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 2, SHORT>, "w4_rows_kernel", table[1], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 4, SHORT>, "w4_rows_kernel", table[2], p, sp, blocks, tiles_m, THREADS, smem, stream);
+}
 template <int P, bool PACKED, int NT, bool DUAL>
 int backward(const W4RowsArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
-  static SmemOptIn table[3];
   const int kblocks = ceil_div(p.w.n_in, CHUNK), tiles = ceil_div(p.w.n_out, TILE_N);
   const long long units = (long long)kblocks * tiles_m;
   const int split = (int)std::max<long long>(1, std::min<long long>(ceil_div(tiles, WARPS), (2LL * SMS) / units));
   sp.cluster = std::min(8, power_below(split));
+  // Long sums of fp32 rows (not of one or two, whose parts have columns of their own: 40000 terms are within 1.3e-7).  Up to eight rows the additions are cheap (16384 x 16384, us: eight
+  // 69.9 -> 75.9, with four times the blocks 81.7).  More rows
+  // and pairs have no registers left for them, and are split over more blocks where 8 of those suffice (16384 x 16384: 16 rows 117 -> 133, with additions 144; 64 rows 445 -> 494, 549;
+  // 8192 x 4096: 64 rows 61.9 -> 67.7, 73.8; pairs of 48 125 -> 105, 146).
+  constexpr bool CHEAP = NT == 1 && !DUAL;
+  bool additions = false;
+  if (P == 3 && !PACKED) {
+    while (!CHEAP && sp.cluster < 8 && ceil_div(tiles, WARPS * sp.cluster) > MOST_IN_ONE) sp.cluster *= 2;
+    additions = ceil_div(tiles, WARPS * sp.cluster) > MOST_IN_ONE;
+  }
   sp.cluster_log2 = log2_of(sp.cluster);
   const int cv = PACKED ? sp.tile_m * P : (NT == 1 ? sp.tile_m : 8);
   const int rows_bytes = WARPS * (DUAL ? 2 : 1) * (PACKED ? 1 : P * NT) * cv * 64;
   const int smem = RING_BYTES + rows_bytes + (DUAL ? 2 : 1) * sp.tile_m * CHUNK * 4;  // ring (the sums over the warps at the end need less), parts, sums of the cluster
   const long long blocks = (long long)kblocks * sp.cluster;
-  if (p.w.group_log2 == 5) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 1>, "w4_rows_kernel", table[0], p, sp, blocks, tiles_m, THREADS, smem, stream);
-  if (p.w.group_log2 == 6) return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 2>, "w4_rows_kernel", table[1], p, sp, blocks, tiles_m, THREADS, smem, stream);
-  return launch_clustered(w4_rows_kernel<P, PACKED, NT, DUAL, 4>, "w4_rows_kernel", table[2], p, sp, blocks, tiles_m, THREADS, smem, stream);
+  if constexpr (P == 3 && !PACKED) {
+    if (additions) return launch_groups<P, PACKED, NT, DUAL, true>(p, sp, blocks, tiles_m, smem, stream);
+  }
+  return launch_groups<P, PACKED, NT, DUAL, false>(p, sp, blocks, tiles_m, smem, stream);
 }
 
 }  // namespace

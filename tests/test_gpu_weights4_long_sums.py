@@ -2,7 +2,8 @@
 
 Tolerance, of the sum of magnitudes, which for positive rows and weights is the result itself.  A matrix instruction adds 16 products to an accumulator and cuts off less than one
 unit in the last place (2^-23) of it.  Kernels for many rows: at most 48 instructions a sum, then one rounding (2^-24) for each of the n / 128 sums, the weight's own roundings below 2^-22:
-2^-23 * 48 + 2^-24 * (n / 128 + 8).
+2^-23 * 48 + 2^-24 * (n / 128 + 8).  Kernels for few rows: as many instructions, or 6 and an addition for every 32 of a warp's outputs, of which each of 8 warps has a share, then sums over warps and
+blocks: 2^-23 * 48 + 2^-24 * (n / 256 + 24).
 """
 import pytest
 import torch
@@ -38,3 +39,23 @@ def test_many_rows(dev, n, m, monkeypatch):
     for got in (gl, gu):
         worst = float(((got.double() - want).abs() / want).max())
         assert worst <= 2.0 ** -23 * 48 + 2.0 ** -24 * (n / 128 + 8), worst
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [2, 8, 100])
+@pytest.mark.parametrize("n", [9000, 20000])
+def test_few_rows(dev, m, n, group, monkeypatch):
+    """100 rows through 4096 columns fill the chip by themselves: a block has all outputs unless sums of many ask for more blocks."""
+    from boundflow_b200 import weights4
+
+    monkeypatch.setattr(weights4, "_many_pays", lambda *a: False)
+    W, w, g = positive(n, 4096, group, dev, n + m + group)
+    a = torch.rand(m, n, generator=g).to(dev)
+    want = a.double() @ w
+    tol = 2.0 ** -23 * 48 + 2.0 ** -24 * (n / 256 + 24)
+    worst = float(((weights4.rows_times_weight4(a, W).double() - want).abs() / want).max())
+    assert worst <= tol, worst
+    lo, up = torch.zeros(m, 4096, device=dev).requires_grad_(), torch.ones(m, 4096, device=dev).requires_grad_()
+    gl, gu = torch.autograd.grad(weights4.interval_linear4(lo, up, W), (lo, up), (a, a))
+    for got in (gl, gu):
+        assert float(((got.double() - want).abs() / want).max()) <= tol
