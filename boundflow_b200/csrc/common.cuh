@@ -129,6 +129,11 @@ inline cudaStream_t as_stream(bf_stream_t s) { return reinterpret_cast<cudaStrea
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // ---- device helpers --------------------------------------------------------
+// max(x, 0) that keeps a NaN (fmaxf would make a bound of zero of it): the results of a wait that ran out, or of weights that hold one, may not pass for bounds.
+__device__ __forceinline__ float relu_of(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(0.f));
+  return x;
+}
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Loads 4 consecutive floats p[idx..idx+3] with a bound `n_valid` (elements of

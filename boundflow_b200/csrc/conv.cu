@@ -73,7 +73,7 @@ __device__ __forceinline__ float2 taps_inside(const IbpConvArgs& g, long long pi
         if (INTERVAL) {
           float d = g.in_b[i];
           if (g.in_mode == BF_IN_LOWER_UPPER) {
-            if (g.relu_in) { c = fmaxf(c, 0.f); d = fmaxf(d, 0.f); }
+            if (g.relu_in) { c = relu_of(c); d = relu_of(d); }
             const float mid = (c + d) * 0.5f;
             d = (d - c) * 0.5f;
             c = mid;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(1024 / TC) conv_tile_kernel(IbpConvArgs g, int
       if (INTERVAL) {
         float b = rb[j];
         if (g.in_mode == BF_IN_LOWER_UPPER) {
-          if (g.relu_in) { a = fmaxf(a, 0.f); b = fmaxf(b, 0.f); }
+          if (g.relu_in) { a = relu_of(a); b = relu_of(b); }
           const float c = (a + b) * 0.5f;
           b = (b - a) * 0.5f;
           a = c;

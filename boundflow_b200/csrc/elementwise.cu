@@ -683,8 +683,8 @@ namespace bf {
 __global__ void interval_relu_kernel(const float* __restrict__ l, const float* __restrict__ u, float* __restrict__ ol,
                                      float* __restrict__ ou, long long n) {
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    ol[i] = fmaxf(l[i], 0.f);
-    ou[i] = fmaxf(u[i], 0.f);
+    ol[i] = relu_of(l[i]);
+    ou[i] = relu_of(u[i]);
   }
 }
 __global__ void interval_add_kernel(const float* __restrict__ al, const float* __restrict__ au, const float* __restrict__ bl,

@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(256) ibp_linear_kernel(IbpArgs g, int chain) {
       float4 b = g.in_b ? load4_guard(g.in_b + (size_t)m * g.K, k, g.K, vK) : make_float4(0.f, 0.f, 0.f, 0.f);
       if (g.in_mode == BF_IN_LOWER_UPPER) {
         if (g.relu_in) {
-          a.x = fmaxf(a.x, 0.f); a.y = fmaxf(a.y, 0.f); a.z = fmaxf(a.z, 0.f); a.w = fmaxf(a.w, 0.f);
-          b.x = fmaxf(b.x, 0.f); b.y = fmaxf(b.y, 0.f); b.z = fmaxf(b.z, 0.f); b.w = fmaxf(b.w, 0.f);
+          a.x = relu_of(a.x); a.y = relu_of(a.y); a.z = relu_of(a.z); a.w = relu_of(a.w);
+          b.x = relu_of(b.x); b.y = relu_of(b.y); b.z = relu_of(b.z); b.w = relu_of(b.w);
         }
         creg = make_float4((a.x + b.x) * 0.5f, (a.y + b.y) * 0.5f, (a.z + b.z) * 0.5f, (a.w + b.w) * 0.5f);
         rreg = make_float4((b.x - a.x) * 0.5f, (b.y - a.y) * 0.5f, (b.z - a.z) * 0.5f, (b.w - a.w) * 0.5f);
@@ -228,7 +228,7 @@ __device__ __forceinline__ void ibp_finish(const IbpArgs& g, int row, int col, f
 }
 __device__ __forceinline__ void centre_radius(const IbpArgs& g, float& a, float& b) {
   if (g.in_mode != BF_IN_LOWER_UPPER) return;
-  if (g.relu_in) { a = fmaxf(a, 0.f); b = fmaxf(b, 0.f); }
+  if (g.relu_in) { a = relu_of(a); b = relu_of(b); }
   const float c = (a + b) * 0.5f;
   b = (b - a) * 0.5f;
   a = c;
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(256) ibp_linear_batched_kernel(const float* __
   float c = 0.f, d = 0.f;
   for (int i = lane; i < n_in; i += 32) {
     float lo = xl[i], up = xu[i];
-    if (relu_in) { lo = fmaxf(lo, 0.f); up = fmaxf(up, 0.f); }
+    if (relu_in) { lo = relu_of(lo); up = relu_of(up); }
     const float wv = w[i];
     c = fmaf(0.5f * (lo + up), wv, c);
     d = fmaf(0.5f * (up - lo), fabsf(wv), d);
