@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import Any, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _lib
 from .network import _cuda_device
@@ -282,6 +283,12 @@ def _check_rows(name: str, x: Any, weight: Any, width: str) -> None:
         raise ValueError(f"{name}: rows of {int(x.shape[-1]) if x.dim() else 0} do not match {weight!r}")
 
 
+def _refuse_tangents(name: str, *tensors: Any) -> None:
+    """A tensor that carries a forward-mode tangent asks for no gradient: without this the launch would drop it."""
+    if _forward._current_level >= 0 and any(torch.is_tensor(t) and t.is_floating_point() and _forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def _check_bias(name: str, bias: Any, weight: Weight4) -> None:
     if bias is not None and (not torch.is_tensor(bias) or bias.dtype not in _TYPES):
         raise TypeError(f"{name} takes an fp32, bf16 or fp16 bias")
@@ -305,6 +312,7 @@ def _placed(t: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable in x and bias."""
+    _refuse_tangents("linear4", x, bias)
     if type(weight) is Weight4 and torch.is_tensor(x) and _ready(x, weight, weight.n_in, bias):
         return _linear(x, weight, bias)
     _check_rows("linear4", x, weight, "n_in")
@@ -326,6 +334,7 @@ def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, 
                      relu_in: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """Bounds of x W^T + bias for lower <= x <= upper (fp32 [..., n_in]); `relu_in` clamps the input at zero first.  Differentiable once, for lower, upper
     and bias (without relu_in)."""
+    _refuse_tangents("interval_linear4", lower, upper, bias)
     if (type(weight) is Weight4 and torch.is_tensor(lower) and torch.is_tensor(upper) and lower.dtype == upper.dtype == torch.float32 and lower.shape == upper.shape
             and _ready(lower, weight, weight.n_in, bias) and _ready(upper, weight, weight.n_in, None) and (bias is None or bias.dtype == torch.float32)):
         return _interval(lower, upper, _lib.IN_LOWER_UPPER, 1 if relu_in else 0, weight, bias)
@@ -355,6 +364,7 @@ def interval_linear4(lower: torch.Tensor, upper: torch.Tensor, weight: Weight4, 
 def rows_times_weight4(A: torch.Tensor, weight: Weight4) -> torch.Tensor:
     """A W for coefficient rows A [..., n_out] in fp32, bf16 or fp16 (sums in fp32, rounded once; beside 16-bit rows each product is held to 2^-17): the
     gradient of `linear4`.  Differentiable in A."""
+    _refuse_tangents("rows_times_weight4", A)
     if type(weight) is Weight4 and torch.is_tensor(A) and _ready(A, weight, weight.n_out, None):
         return _rows(A, weight)
     _check_rows("rows_times_weight4", A, weight, "n_out")
