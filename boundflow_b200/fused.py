@@ -20,6 +20,7 @@ import torch
 
 from . import _lib
 from .network import _pair, dense_conv_weight
+from .weights4 import Weight4
 
 
 @dataclass(frozen=True)
@@ -78,11 +79,13 @@ class CudaFusedCrownExecutor:
         tensors = [request.A_u, request.A_l, request.alpha_u, request.alpha_l, request.beta_u, request.beta_l, request.weight]
         if request.bias is not None:
             tensors.append(request.bias)
-        ok = all(t.device.type == "cuda" and t.dtype == torch.float32 and t.is_contiguous() and not t.requires_grad for t in tensors)
+        ok = all(torch.is_tensor(t) and t.device.type == "cuda" and t.dtype == torch.float32 and t.is_contiguous() and not t.requires_grad for t in tensors)
         return bool(ok)
 
     def run(self, request: Any, *, stream: Optional[torch.cuda.Stream] = None) -> FusedReluAffineResult:
         device = request.A_u.device
+        if isinstance(request.weight, Weight4):
+            raise NotImplementedError("a fused region reads a dense weight; this one is held in 4 bits (Weight4.dense() makes one)")
         if device.type != "cuda":
             raise RuntimeError("CudaFusedCrownExecutor needs CUDA tensors")
         st = stream if stream is not None else torch.cuda.current_stream(device)

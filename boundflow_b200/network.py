@@ -147,7 +147,9 @@ class CudaChain:
         def dev(name: str, attrs: Any = None) -> torch.Tensor:
             t = params[name]
             if isinstance(t, Weight4):
-                raise NotImplementedError(f"'{name}' is held in 4 bits: the fused sweeps read dense weights (the functions of crown.py and dag.py take it)")
+                raise NotImplementedError(
+                    f"'{name}' is held in 4 bits, and ibp_trace, bound_split_domains and run_crown_intermediate_mlp read dense weights (Weight4.dense() makes one); "
+                    "run_ibp, run_crown_ibp_mlp, run_alpha_crown_mlp, run_alpha_beta_crown_mlp and CudaQueryRuntime take it as it is")
             given = t if torch.is_tensor(t) else torch.as_tensor(t)
             out = dense_conv_weight(given.detach().to(device=self.device, dtype=torch.float32).contiguous(), attrs)
             if torch.is_tensor(t) and out.data_ptr() != t.data_ptr():

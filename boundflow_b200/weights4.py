@@ -1,8 +1,10 @@
 """Linear layers whose weights are held in 4 bits with a scale for each group of columns.
 
-`Weight4` stands where a Linear layer's weight does: in the `params` of a module that `CudaTaskExecutor.run_ibp`, `run_crown_ibp_mlp`,
-`run_alpha_beta_crown_mlp` and the other whole-query functions bound (such modules take the graph path of `dag.py`), as the weight of
-`CudaIntervalDomain.affine_transformer`, and in the products below:
+`Weight4` stands where a Linear layer's weight does: in the `params` of a module that `CudaTaskExecutor.run_ibp`, `forward_ibp_trace_mlp`, `run_crown_ibp_mlp`
+(`_from_forward_trace` and with ReLU influence too), `run_alpha_crown_mlp`, `run_alpha_beta_crown_mlp`, `first_layer_certificate` and `CudaQueryRuntime` bound (such modules
+take the graph path of `dag.py`; L1 and L2 balls and the certificate make a dense copy of the first layer in every call), as the weight of
+`CudaIntervalDomain.affine_transformer`, and in the products below.  `ibp_trace`, `bound_split_domains`, `run_crown_intermediate_mlp` and fused regions read dense
+weights and refuse it; `dense()` makes one.
 
     linear4(x, weight, bias)                   x W^T + b, with gradients for x and bias (the weight is frozen)
     interval_linear4(lower, upper, weight, b)  bounds of it over boxes, with gradients for lower, upper and bias

@@ -21,3 +21,36 @@ def test_forward_mode_tangents_are_refused():
                      lambda: rows_times_weight4(da, w)):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def chain():
+    from boundflow_b200.ir import BFTaskModule, BoundTask, TaskKind, TaskOp
+
+    ops = [TaskOp("linear", "l1", ["x", "W"], ["y"])]
+    task = BoundTask(task_id="t", kind=TaskKind.INTERVAL_IBP, ops=ops, input_values=["x"], output_values=["y"])
+    return BFTaskModule([task], "t", {"params": {"W": weight()}})
+
+
+def test_chains_say_what_takes_a_4_bit_weight():
+    from boundflow_b200.csrc import build
+    from boundflow_b200.network import CudaChain
+
+    build.build()
+    with pytest.raises(NotImplementedError, match="bound_split_domains.*run_crown_intermediate_mlp.*run_alpha_beta_crown_mlp"):
+        CudaChain(chain(), (40,), torch.device("cuda", 0))
+
+
+def test_fused_regions_refuse_a_4_bit_weight():
+    from types import SimpleNamespace
+
+    from boundflow_b200.csrc import build
+    from boundflow_b200.fused import CudaFusedCrownExecutor
+
+    build.build()
+    rows, line = torch.zeros(1, 2, 4), torch.zeros(1, 4)
+    request = SimpleNamespace(kind="linear", A_u=rows, A_l=rows, alpha_u=line, alpha_l=line, beta_u=line, beta_l=line, weight=weight(), bias=None, input_shape=(40,), output_shape=(4,),
+                              attrs={})
+    executor = CudaFusedCrownExecutor()
+    assert executor.supports(request, SimpleNamespace()) is False
+    with pytest.raises(NotImplementedError, match="4 bits"):
+        executor.run(request)
