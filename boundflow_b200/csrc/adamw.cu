@@ -206,7 +206,8 @@ __device__ __forceinline__ void cut(float (&x)[8]) {
 }
 
 // Root and quotient of the step itself need no more than the approximations' 2^-22: the step is far below the parameter.  Numbers below the normal range
-// count as zero in them, which an eps above 1e-18 covers.
+// count as zero in them: a root below 2^-63, times the correction 1 / sqrt(1 - b2^t), which is below 2^-22 of an eps from LEAST_EPS times that correction on.
+constexpr float LEAST_EPS = 4.6e-13f;
 __device__ __forceinline__ float quotient(float m, float v, float root, float eps) {
   float s, q;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_
         v[i] = __fadd_rn(__fmul_rn(c.b2, v[i]), __fmul_rn(__fmul_rn(c.c2, gi), gi));
       }
       const float step = -e.lr * rate, decay = e.decay;
-      if (c.eps > 1e-18f) {
+      if (c.eps > LEAST_EPS * root) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = fmaf(step, quotient(m[i], v[i], root, c.eps), p[i] * decay);
       } else {

@@ -1,0 +1,26 @@
+"""AdamW where numbers leave the normal range: second moments below it, an eps that does not cover them.  The moments are taken from the optimiser (they are tested bit for bit
+elsewhere); the step from them is formed in 64 bits, with the tolerance of `check_params`."""
+import pytest
+import torch
+
+from tests.test_gpu_adamw import check_params, dev  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1.1e-18, 2e-18, 1e-16, 1e-13, 1e-8])
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.5, 0.9999), (0.0, 0.0)])
+def test_second_moments_below_the_normal_range(dev, bits, eps, betas):
+    from boundflow_b200.optim import AdamW
+
+    grad = torch.cat([torch.full((256,), g) for g in (3.4e-18, 1e-18, 3e-17, 1e-15, 1e-10, 2e-19)]).to(dev)
+    p = torch.zeros_like(grad)
+    opt = AdamW([p], lr=1.0, betas=betas, eps=eps, weight_decay=0.0, state_bits=bits)
+    before = p.clone()
+    opt.step([grad])
+    eps32, g = float(torch.tensor(eps)), grad.double()
+    c1, c2 = (float(torch.tensor(1 - b)) for b in betas)
+    m = (c1 * g).float().double()
+    v = ((c2 * g).float().double() * g).float().double()  # each product rounded by itself
+    check_params(p, before, m, v, 1, 1.0, 0.0, betas, eps32)
