@@ -8,6 +8,20 @@ from tests.test_gpu_adamw import check_params, dev  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
+def test_roundings_of_a_step_with_32_bit_moments(dev):
+    """From p = 0, with lr and both corrections powers of two, a step is three roundings of at most 2^-24 each: sqrt(v), that plus eps, and the quotient."""
+    from boundflow_b200.optim import AdamW
+
+    g = torch.Generator("cpu").manual_seed(3)
+    grad = (torch.randn(200000, generator=g) * torch.exp2(20 * torch.rand(200000, generator=g) - 10)).to(dev)
+    p = torch.zeros_like(grad)
+    AdamW([p], lr=2.0 ** -8, betas=(0.5, 0.75), eps=2.0 ** -30, weight_decay=0.0).step([grad])  # 1 / (1 - 0.5) = 2, 1 / sqrt(1 - 0.75) = 2
+    x = grad.double()
+    v = ((0.25 * x).float().double() * x).float().double()
+    want = -(2.0 ** -7) * (0.5 * x) / (2 * v.sqrt() + 2.0 ** -30)
+    assert float(((p.double() - want) / want).abs().max()) <= 3.0 * 2.0 ** -24 * 1.000001
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("eps", [1.1e-18, 2e-18, 1e-16, 1e-13, 1e-8])
 @pytest.mark.parametrize("betas", [(0.9, 0.999), (0.5, 0.9999), (0.0, 0.0)])
