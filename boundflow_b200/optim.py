@@ -45,9 +45,7 @@ class AdamW:
                  *, state_bits: int = 32):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits={state_bits!r}: 8 or 32")
-        b1, b2 = (float(b) for b in betas)
-        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not float(eps) >= 0.0:
-            raise ValueError(f"betas={betas!r}, eps={eps!r}: betas in [0, 1) and eps >= 0 are wanted")
+        self.betas, self.eps = self._constants(betas, eps)
         given = [params] if torch.is_tensor(params) else list(params)
         groups = [dict(g) for g in given] if given and isinstance(given[0], dict) else [{"params": given}]
         self.param_groups: List[Dict[str, Any]] = []
@@ -72,7 +70,7 @@ class AdamW:
                 raise ValueError(f"AdamW: parameter {k} is not contiguous")
         self._refuse_overlap()
         self._options()
-        self.betas, self.eps, self.state_bits, self.device = (b1, b2), float(eps), state_bits, self._params[0].device
+        self.state_bits, self.device = state_bits, self._params[0].device
         self._sizes, self._types = [p.numel() for p in self._params], [p.dtype for p in self._params]
         self._bytes, self._one_type = [n * _SIZE[t] for n, t in zip(self._sizes, self._types)], len(set(self._types)) == 1
         self._inference = any(p.is_inference() for p in self._params)
@@ -89,6 +87,23 @@ class AdamW:
         self._table["n"], self._table["first"] = self._sizes, self._first[:-1]
 
     # ---- checks -----------------------------------------------------------------
+    @staticmethod
+    def _constants(betas: Any, eps: Any) -> Tuple[Tuple[float, float], float]:
+        b1, b2 = (float(b) for b in betas)
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not float(eps) >= 0.0:
+            raise ValueError(f"betas={betas!r}, eps={eps!r}: betas in [0, 1) and eps >= 0 are wanted")
+        return (b1, b2), float(eps)
+
+    def _check_moments(self, step: int, moments: Dict[str, torch.Tensor]) -> List[str]:
+        names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exponent", "exp_avg_sq_exponent"] if self.state_bits == 8 else [])
+        if set(moments) != set(names) or int(step) < 0:
+            raise ValueError(f"load_flat_moments: step >= 0 and {names} are wanted, got step={step} and {sorted(moments)}")
+        for name in names:
+            buf, t = getattr(self, name), moments[name]
+            if t.shape != buf.shape or t.dtype != buf.dtype:
+                raise ValueError(f"load_flat_moments: {name} is {tuple(t.shape)} {t.dtype}, {tuple(buf.shape)} {buf.dtype} is wanted")
+        return names
+
     def _refuse_overlap(self) -> None:
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), k) for k, p in enumerate(self._params) if p.numel())
         for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
@@ -195,13 +210,7 @@ class AdamW:
 
     def load_flat_moments(self, step: int, **moments: torch.Tensor) -> None:
         """Sets the step count and the flat buffers (`exp_avg`, `exp_avg_sq` and, for 8-bit states, `exp_avg_exponent`, `exp_avg_sq_exponent`)."""
-        names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exponent", "exp_avg_sq_exponent"] if self.state_bits == 8 else [])
-        if set(moments) != set(names) or int(step) < 0:
-            raise ValueError(f"load_flat_moments: step >= 0 and {names} are wanted, got step={step} and {sorted(moments)}")
-        for name in names:
-            buf, t = getattr(self, name), moments[name]
-            if t.shape != buf.shape or t.dtype != buf.dtype:
-                raise ValueError(f"load_flat_moments: {name} is {tuple(t.shape)} {t.dtype}, {tuple(buf.shape)} {buf.dtype} is wanted")
+        names = self._check_moments(step, moments)
         for name in names:
             getattr(self, name).copy_(moments[name])
         self._set_step(int(step))
@@ -215,7 +224,12 @@ class AdamW:
     def load_state_dict(self, state: Dict[str, Any]) -> None:
         if state["state_bits"] != self.state_bits or list(state["sizes"]) != self._sizes or len(state["groups"]) != len(self.param_groups):
             raise ValueError("AdamW.load_state_dict: the state is of other tensors, groups or state_bits")
-        self.betas, self.eps = tuple(state["betas"]), float(state["eps"])
+        groups = [{"lr": float(g["lr"]), "weight_decay": float(g["weight_decay"])} for g in state["groups"]]
+        if not all(v >= 0.0 for g in groups for v in g.values()):
+            raise ValueError(f"AdamW.load_state_dict: groups {groups}; lr and weight_decay have to be >= 0")
+        betas, eps = self._constants(state["betas"], state["eps"])
+        self._check_moments(state["step"], state["moments"])
+        self.betas, self.eps = betas, eps  # (from here on nothing is refused: a state that is leaves the optimiser as it was)
         self.load_flat_moments(state["step"], **state["moments"])
-        for g, s in zip(self.param_groups, state["groups"]):
+        for g, s in zip(self.param_groups, groups):
             g.update(s)

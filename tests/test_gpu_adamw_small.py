@@ -1,4 +1,4 @@
-"""AdamW where numbers leave the normal range: second moments below it, an eps that does not cover them.  The moments are taken from the optimiser (they are tested bit for bit
+"""AdamW where numbers leave the normal range (second moments below it, an eps that does not cover them), and states that are refused.  The moments are taken from the optimiser (they are tested bit for bit
 elsewhere); the step from them is formed in 64 bits, with the tolerance of `check_params`."""
 import pytest
 import torch
@@ -38,3 +38,30 @@ def test_second_moments_below_the_normal_range(dev, bits, eps, betas):
     m = (c1 * g).float().double()
     v = ((c2 * g).float().double() * g).float().double()  # each product rounded by itself
     check_params(p, before, m, v, 1, 1.0, 0.0, betas, eps32)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_state_changes_nothing(dev, bits):
+    from boundflow_b200.optim import AdamW
+
+    def fresh():
+        g = torch.Generator("cpu").manual_seed(7)
+        p = torch.randn(500, generator=g).to(dev)
+        opt = AdamW([p], lr=0.01, state_bits=bits)
+        opt.step([torch.randn(500, generator=g).to(dev)])
+        return opt
+
+    opt, twin = fresh(), fresh()
+    good = opt.state_dict()
+    moments = {k: v.clone() for k, v in good["moments"].items()}
+    wrong = dict(moments, exp_avg=moments["exp_avg"][:256])
+    for change in ({"moments": wrong, "betas": (0.1, 0.2), "eps": 1.0}, {"betas": (0.5, 1.5)}, {"betas": (0.5, float("nan"))}, {"eps": -1.0, "betas": (0.1, 0.2)},
+                   {"step": -1, "betas": (0.1, 0.2)}, {"groups": [{"lr": -1.0, "weight_decay": 0.0}], "betas": (0.1, 0.2)}, {"moments": {}, "eps": 1.0}):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(dict(good, **change))
+        assert (opt.betas, opt.eps, opt.param_groups[0]["lr"]) == (twin.betas, twin.eps, twin.param_groups[0]["lr"])
+    grad = torch.linspace(-1, 1, 500, device=dev)
+    opt.step([grad])
+    twin.step([grad])
+    assert torch.equal(opt.param_groups[0]["params"][0], twin.param_groups[0]["params"][0])
+    assert all(torch.equal(a, b) for a, b in zip(opt.flat_moments(), twin.flat_moments()))
