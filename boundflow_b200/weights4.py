@@ -25,6 +25,7 @@ from torch.autograd import forward_ad as _forward
 from . import _lib
 from .network import _cuda_device
 
+_MOST_ROWS, _MOST_SIDE = 2 ** 31 - 1, 2 ** 30  # of a call, of a weight: the library counts them in 32 bits
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 
 
@@ -47,6 +48,8 @@ class Weight4:
         group = padded // groups if groups else 0
         if int(scales.shape[1]) != n_out or groups == 0 or group * groups != padded or not padded - group < n_in <= padded:
             raise ValueError(f"Weight4: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {n_in} weights")
+        if n_out > _MOST_SIDE or n_in > _MOST_SIDE:
+            raise ValueError(f"Weight4: {n_out} x {n_in} weights (at most 2^30 a side)")
         if group < 32 or group > 1 << 20 or group & (group - 1):
             raise ValueError(f"Weight4: groups of {group} weights (a power of two from 32 to 2^20 is wanted)")
         if codes.device != scales.device:
@@ -107,6 +110,8 @@ def quantise_weight4(W: torch.Tensor, group: int = 128) -> Weight4:
     group = int(group)
     if W.dim() != 2 or W.shape[0] < 1 or W.shape[1] < 1:
         raise ValueError(f"quantise_weight4: a weight [n_out, n_in] is wanted, got {tuple(W.shape)}")
+    if max(W.shape) > _MOST_SIDE:
+        raise ValueError(f"quantise_weight4: {tuple(W.shape)} weights (at most 2^30 a side)")
     if group < 32 or group > 1 << 20 or group & (group - 1):
         raise ValueError(f"quantise_weight4: groups of {group} weights (a power of two from 32 to 2^20 is wanted)")
     device = _device_of(W)
@@ -283,6 +288,8 @@ def _check_rows(name: str, x: Any, weight: Any, width: str) -> None:
         raise TypeError(f"{name} takes fp32, bf16 or fp16 tensors")
     if x.dim() < 1 or x.shape[-1] != getattr(weight, width):
         raise ValueError(f"{name}: rows of {int(x.shape[-1]) if x.dim() else 0} do not match {weight!r}")
+    if x.numel() > _MOST_ROWS * x.shape[-1]:
+        raise ValueError(f"{name}: {x.numel() // x.shape[-1]} rows (at most 2^31 - 1 in a call)")
 
 
 def _refuse_tangents(name: str, *tensors: Any) -> None:
@@ -301,7 +308,7 @@ def _check_bias(name: str, bias: Any, weight: Weight4) -> None:
 def _ready(x: Any, weight: Any, width: int, bias: Any) -> bool:
     """Whether a call can go straight to its launch: rows [M, width] and bias as the kernels read them, on the weight's device, and no gradient asked for.
     (All else takes the checks and copies below; microseconds that a small layer's kernel does not take.)"""
-    return (x.is_cuda and x.dim() == 2 and x.shape[1] == width and x.dtype in _TYPES and x.is_contiguous() and x.get_device() == weight.codes.get_device()
+    return (x.is_cuda and x.dim() == 2 and x.shape[1] == width and x.shape[0] <= _MOST_ROWS and x.dtype in _TYPES and x.is_contiguous() and x.get_device() == weight.codes.get_device()
             and not (x.requires_grad and torch.is_grad_enabled())
             and (bias is None or (torch.is_tensor(bias) and bias.is_cuda and bias.dim() == 1 and bias.shape[0] == weight.n_out and bias.dtype in _TYPES and bias.is_contiguous()
                                   and bias.get_device() == x.get_device() and not (bias.requires_grad and torch.is_grad_enabled()))))

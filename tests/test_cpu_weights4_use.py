@@ -54,3 +54,18 @@ def test_fused_regions_refuse_a_4_bit_weight():
     assert executor.supports(request, SimpleNamespace()) is False
     with pytest.raises(NotImplementedError, match="4 bits"):
         executor.run(request)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """The library takes 32-bit counts: 2^32 + 5 rows would be 5.  (Expanded tensors: no memory behind them.)"""
+    from boundflow_b200.weights4 import interval_linear4, linear4, quantise_weight4, rows_times_weight4
+
+    w, many = weight(), 2 ** 32 + 5
+    x, a = torch.zeros(1, 40).expand(many, 40), torch.zeros(1, 4).expand(many, 4)
+    for call in (lambda: linear4(x, w), lambda: linear4(x.unsqueeze(0), w), lambda: interval_linear4(x, x, w), lambda: rows_times_weight4(a, w),
+                 lambda: linear4(torch.zeros(1, 40).expand(2 ** 31, 40), w)):
+        with pytest.raises(ValueError, match="at most 2.31 - 1"):
+            call()
+    for shape in ((many, 40), (40, many), (2 ** 30 + 1, 1)):
+        with pytest.raises(ValueError, match="at most 2.30"):
+            quantise_weight4(torch.zeros(1, 1).expand(shape))
