@@ -176,7 +176,8 @@ __device__ __forceinline__ void cluster_barrier() {
 template <typename Args>
 int launch_clustered(void (*kernel)(Args, Split), const char* name, SmemOptIn& table, const Args& p, const Split& sp, long long blocks, int tiles_m, int threads,
                      int smem, cudaStream_t stream) {
-  const int rc = ensure_dynamic_smem(kernel, smem, table, name);
+  // (the most that any call asks for: with each call's own size, the limit of a first call could be lowered by that of another thread's before its launch)
+  const int rc = ensure_dynamic_smem(kernel, 227 * 1024, table, name);
   if (rc != BF_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, tiles_m);
