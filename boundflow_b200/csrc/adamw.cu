@@ -145,7 +145,8 @@ __device__ __forceinline__ Eight<float> rounded<float>(const float (&x)[8]) {
 // are multiplications (which run beside it), and signs and zeros are dealt with for four codes at a time.
 constexpr int M_FIELDS = 15, V_FIELDS = 31;  // powers of two below the block's exponent
 
-// The 32 random bits of the four elements at `place` (a multiple of four, so that the first mixing is the same for them but for the last two bits).
+// The 32 random bits of the four elements at `place` (a multiple of four, so that the first mixing is the same for them but for the last two bits).  Shifts and products with odd
+// constants, arbitrary ones: what is asked of them is that roundings up and down balance over elements and steps, to which a test of the moments' means holds them.
 __device__ __forceinline__ void rounding_noise(uint32_t place, uint32_t key, uint32_t (&noise)[4]) {
   const uint32_t first = place ^ key, mixed = first ^ (first >> 16);
 #pragma unroll

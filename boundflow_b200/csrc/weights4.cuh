@@ -27,6 +27,19 @@ __device__ __forceinline__ void store_any(void* p, int type, long long i, float 
   else static_cast<__half*>(p)[i] = __float2half(v);
 }
 
+// Codes in bits 0-3 and 16-19 of `w`, minus 8, as two bfloat16: 0x4300 | code is 128 + code, since 128 has its last mantissa bit at 1 (building a float from an integer's bits so is common practice).  ("And, or" is one instruction where one of the two constants is
+// in a register, which the compiler does not do by itself: the integer pipe, 64 lanes a clock, is what these kernels fill first.)
+__device__ __forceinline__ uint32_t weights_of(uint32_t w) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
+  const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // y = x W^T + bias, or with `b` the bounds of it over boxes.
 struct W4LinearArgs {
   W4 w;

@@ -44,9 +44,6 @@ __device__ __forceinline__ Eight<P> load8(const void* base, long long at, int le
   }
   return e;
 }
-__device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
 
 // Digits (P = DIGITS): up to four 16-bit rows as whole numbers of four 8-bit digits, counted in 2^(e - 156) with e the biased exponent of the largest of the row's
 // columns that share a scale (128 of them at most).  A bfloat16 number is held exactly down to 2^-22 of that largest, a half down to 2^-19.  The codes

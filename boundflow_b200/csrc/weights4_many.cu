@@ -100,17 +100,6 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(0u)
       : "memory");
 }
-__device__ __forceinline__ void put16(uint32_t at, const uint32_t (&v)[4]) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-}
-// Codes in bits 0-3 and 16-19, minus 8, as two bfloat16 (0x4300 | code is 128 + code).
-__device__ __forceinline__ uint32_t pair_of(uint32_t w) {
-  uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
-  const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
 // ---- images of the rows ----------------------------------------------------------------
@@ -123,7 +112,7 @@ struct ImageArgs {
   int type, take, mode, relu_in, M, n, tile_m, steps;
 };
 // [row tile][64 columns][part][row of the tile][128 bytes, in eights, the eight e of row r in place e ^ (r % 8)].  FORWARD: the eights in the order 0 4 1 5 2 6 3 7 that
-// `pair_of` gives the codes of a word in.  What is outside the rows is zero.  Eight columns of a row a thread.
+// `weights_of` gives the codes of a word in.  What is outside the rows is zero.  Eight columns of a row a thread.
 template <int PARTS, bool FORWARD>
 __global__ void __launch_bounds__(256) w4_rows_images_kernel(const ImageArgs p) {
   const long long row_eights = (long long)p.steps * 8, rows = (long long)((p.M + p.tile_m - 1) / p.tile_m) * p.tile_m, total = rows * row_eights;
@@ -311,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
             some |= keep != 0xffffffffu;
             v[j] &= keep;
           }
-          if (some) put16(at + i, v);
+          if (some) put16(at + i, v[0], v[1], v[2], v[3]);
         }
       };
       const bool one = elected();
@@ -495,11 +484,11 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
               uint32_t q[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                q[i] = pair_of(word[e] >> (4 * i));
+                q[i] = weights_of(word[e] >> (4 * i));
                 if (absolute) q[i] &= 0x7fff7fffu;
               }
               if (FORWARD) {
-                put16(at, q);
+                put16(at, q[0], q[1], q[2], q[3]);
               } else {
                 uint32_t part[WP][4];
 #pragma unroll
@@ -520,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
                   }
                 }
 #pragma unroll
-                for (int k = 0; k < WP; ++k) put16(at + k * A_BYTES, part[k]);
+                for (int k = 0; k < WP; ++k) put16(at + k * A_BYTES, part[k][0], part[k][1], part[k][2], part[k][3]);
               }
             }
           }

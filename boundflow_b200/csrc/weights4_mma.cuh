@@ -38,15 +38,6 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool valid)
 __device__ __forceinline__ void copies_begin() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// Codes in bits 0-3 and 16-19 of `w`, minus 8, as two bfloat16: 0x4300 | code is 128 + code.  ("And, or" is one instruction where one of the two constants is
-// in a register, which the compiler does not do by itself: the integer pipe, 64 lanes a clock, is what these kernels fill first.)
-__device__ __forceinline__ uint32_t weights_of(uint32_t w) {
-  uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
-  const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
