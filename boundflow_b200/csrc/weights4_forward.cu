@@ -309,8 +309,8 @@ __device__ __forceinline__ void add_rest(const W4LinearArgs& p, int first, int e
 // P parts of a row, side by side in the columns of NT tiles (PACKED) or an instruction each for NT tiles of 8 rows; DUAL: W c and |W| r; F: steps of 32 columns
 // that share a scale (1, 2, or 4 and more).
 //
-// Bounds and measurements (B200, back to back on inputs larger than the L2 cache's share).  One bf16 row through 16384 x 16384: 31.4 us, 4.5 TB/s of codes, scales and
-// rows (69% of a plain copy); issue slots are at 55%, DRAM at 52%, and a launch of nothing but clusters costs 3 to 4 us of it.  Boxes of 4 through 8192 x 8192: 25 us,
+// Bounds and measurements (B200, back to back on inputs larger than the L2 cache's share).  One bf16 row through 16384 x 16384: 31.7 us, 4.5 TB/s of codes, scales and
+// rows (69% of a plain copy; 123 to 182 us where digits leave a rest in every group); issue slots are at 55%, DRAM at 52%, and a launch of nothing but clusters costs 3 to 4 us of it.  Boxes of 4 through 8192 x 8192: 25 us,
 // 1.5 TB/s; two products of three parts keep the tensor cores 35% busy, the rest is waits of 16 warps an SM (128 registers each).  16 bf16 rows
 // through 8192 x 4096: 12.3 us.  Rings of 2 and 4 stages, three blocks an SM, and columns split twice or four times as finely were slower or equal.
 template <int P, bool PACKED, int NT, bool DUAL, int F>

@@ -18,10 +18,10 @@
 // Waits are bounded: where one runs out, the block raises the status word, frees its tensor memory and stores NaN.
 //
 // Bounds and measurements (B200, images included).  4096 bf16 rows through 8192 x 4096: 319 us, 861 TFLOP/s (half of the measured rate of a library's plain product); fp32 rows, three
-// products for one, 624 us (1320 TFLOP/s of bfloat16 products); back, bf16 637 us (two products: 862), fp32 1415 us (six: 1165).  Of a stage of x W^T with 256 bf16 rows (512 clocks of
+// products for one, 617 us (1340 TFLOP/s of bfloat16 products); back, bf16 619 us (two products: 888), fp32 1387 to 1470 us (six: 1120 to 1190), 2.7 ms where every number is infinite.  Of a stage of x W^T with 256 bf16 rows (512 clocks of
 // products) 950 clocks are taken: eight warps need 730 of them for their sums, unpacking 570, issuing 380; beginning and end of a block are another 5 us that nothing hides.  Back, three pairs unpack a
 // stage in 1300 clocks and hold its slot meanwhile.  What was tried: the products issued by a thread that also unpacks (twice the time), by a thread chosen by its number instead of
-// elect.sync (41 us for 64 rows, 31 now), eight warps that both unpack and sum (528 us for 4096 rows, 319 now).
+// elect.sync (41 us for 64 rows, 31 now), sums back of one stage of fp32 rows (7e-7 off instead of 1.1e-6, 5 % slower), eight warps that both unpack and sum (528 us for 4096 rows, 319 now).
 #include <math.h>
 
 #include <algorithm>

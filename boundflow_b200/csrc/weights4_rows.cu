@@ -8,7 +8,7 @@ namespace {
 // into the rows: a[m, n] * scale[group, n], rounded to 32 bits and split into parts, by each warp for the outputs it reads.
 // Columns are the instruction's rows: lane (g, t) takes half a word (four columns) of each of the outputs 2t, 2t + 1, 2t + 8, 2t + 9.
 //
-// Measured (B200): nine fp32 rows back through 4096 x 4096 12.4 us, 16 bf16 rows through 8192 x 4096 18.1, one bf16 row through 16384 x 16384 49 us (2.9 TB/s).  With more than a
+// Measured (B200): nine fp32 rows back through 4096 x 4096 12.0 us, 16 bf16 rows through 8192 x 4096 18.1, one bf16 row through 16384 x 16384 48 us (2.9 TB/s).  With more than a
 // row or two the tensor cores are 41% and the issue slots 49% busy with 16 warps an SM; with one row the parts, which each warp makes for every 32 outputs, and four
 // loads of shared memory for 1024 codes bound it.
 //

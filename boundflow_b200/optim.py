@@ -35,7 +35,8 @@ class AdamW:
     the tensor's type, or any of the three beside fp32 tensors.
 
     `state_bits=8` holds the moments in a byte each with an exponent for every 256 elements (1.004 bytes instead of 4): exponent and 3 mantissa bits,
-    rounded up or down in proportion by a hash of element and step, so that two runs give the same bits.  A block whose gradients hold an infinity
+    rounded up or down in proportion by a hash of element and step, so that two runs give the same bits; the step's root and quotient are good to 2^-22 then (with 32 bits rounded to the
+    nearest).  A block whose gradients hold an infinity
     or a NaN is NaN from then on, as its parameters are.
 
     The step count is on the device: a step that was captured into a graph counts as it is replayed (with the gradients' memory and lr of

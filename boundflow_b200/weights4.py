@@ -14,6 +14,9 @@ weights and refuse it; `dense()` makes one.
 The reference holds all weights in 32 bits; the bounds are those of the network whose weights the codes and scales stand for, computed as
 `bf_ibp_linear` and `bf_crown_relu_linear_bwd` compute them for dense weights.  Like the rest of the package the functions queue their work on the current
 stream of the tensors' device; tensors on the CPU are copied to the current CUDA device and results returned on the device the inputs came from.
+
+Forward, a sum over at most 128 columns of one group is scaled when it is complete, so inputs of 1e35 and more may overflow it whatever the scale.  Infinity times a zero weight is
+NaN, as are infinities of both signs in one sum.  Waits on the device are bounded: where one runs out, the results concerned are NaN, and so are all bounds that follow from them.
 """
 from __future__ import annotations
 
@@ -320,7 +323,8 @@ def _placed(t: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 
 def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable in x and bias."""
+    """x W^T + bias for x [..., n_in] in fp32, bf16 or fp16 (sums in fp32, rounded once to x's type).  Differentiable in x and bias; beside 16-bit rows each
+    product of the gradient of x is held to 2^-17 (`rows_times_weight4`)."""
     _refuse_tangents("linear4", x, bias)
     if type(weight) is Weight4 and torch.is_tensor(x) and _ready(x, weight, weight.n_in, bias):
         return _linear(x, weight, bias)

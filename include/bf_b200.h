@@ -731,7 +731,8 @@ int bf_chain_alpha_beta_crown_shared_reduce(const bf_chain* chain,
  *                        gradients, type) bytes (about 256 MB at most, or what 256 rows need; 0 for sizes or types that there are none of) on a 128-byte boundary.  Its first int is zero afterwards; where it is not, a
  *                        wait on the device ran out and the results concerned are NaN.
  *   bf_w4_many_pays      whether that is expected to be faster for these sizes (backward: rows and gradients; pair: interval and its gradient).
- * A sum over the codes of one group is scaled when it is complete: products of 2^124 / group and more overflow.
+ * A sum over the codes of one group (at most 128 columns) is scaled when it is complete: inputs of 2^124 / 128 and more may overflow it whatever the scale.
+ * Infinities and NaN meet their own weights: infinity times a zero weight is NaN, and so are infinities of both signs in one sum.
  *   bf_rows_dot          d [M] = (accumulate: +=) A [M,n] . bias [n]: the bias term of a coefficient row.
  *   bf_column_sums       out [n] = sum over the M rows of A, in a fixed order: the gradient of a bias. */
 int bf_w4_quantise(const void* W, int type, uint8_t* codes, float* scales, int n_out, int n_in, int group, bf_stream_t stream);
