@@ -8,8 +8,8 @@
 //   x W^T: codes minus 8 are exact in bfloat16, and so are the rows in one part (bf16), two (fp16) or three (fp32), as in weights4_mma.cuh.  The sum over the
 //     columns that share a scale (at most 128 of them) is taken on the tensor cores, into one of two accumulators; from there the eight warps add it, times the scale,
 //     to sums in their registers while the other is filled.
-//   a W: the scale belongs to the summed index, so it goes into the weight: scale * (code - 8) as a sum of two bfloat16 numbers (16-bit rows: off by 2^-17 and, the scale being
-//     held in two parts then, 2^-18), or three (fp32 rows), rounded to the nearest each, and products of parts below 2^-17 (2^-26) of the whole are left out.  Tensor-memory accumulators truncate, by half a unit in the last
+//   a W: the scale belongs to the summed index, so it goes into the weight: scale * (code - 8) as a sum of two bfloat16 numbers (16-bit rows: off by 2^-17 at most) or
+//     three (fp32 rows), rounded to the nearest each.  All products of parts are taken beside 16-bit rows; beside fp32 rows six of nine, what is left out is below 2^-24 of the whole.  Tensor-memory accumulators truncate, by half a unit in the last
 //     place of the running sum for every 16 terms of a product and always in the same direction, so a sum ends after `back_stages` and is added to the registers in the same way
 //     (fp32 rows of 1024 to 65536 terms against 64 bits, 2-norm: 1.1e-6 to 1.2e-6; 8192 terms in one sum 5.3e-5, the FP32 kernel on the dense weight 5e-7 to 4e-6).  A weight's
 //     second part would make NaN of a row's infinity, so where a stage's image holds numbers that are not finite (a bit says so) the image as it is meets the weights' first parts, and a
@@ -18,7 +18,7 @@
 // Waits are bounded: where one runs out, the block raises the status word, frees its tensor memory and stores NaN.
 //
 // Bounds and measurements (B200, images included).  4096 bf16 rows through 8192 x 4096: 319 us, 861 TFLOP/s (half of the measured rate of a library's plain product); fp32 rows, three
-// products for one, 617 us (1340 TFLOP/s of bfloat16 products); back, bf16 619 us (two products: 888), fp32 1387 to 1470 us (six: 1120 to 1190), 2.7 ms where every number is infinite.  Of a stage of x W^T with 256 bf16 rows (512 clocks of
+// products for one, 617 us (1340 TFLOP/s of bfloat16 products); back, bf16 616 us (two products: 892), fp16 794 (four), fp32 1387 to 1470 us (six: 1120 to 1190), 2.7 ms where every number is infinite.  Of a stage of x W^T with 256 bf16 rows (512 clocks of
 // products) 950 clocks are taken: eight warps need 730 of them for their sums, unpacking 570, issuing 380; beginning and end of a block are another 5 us that nothing hides.  Back, three pairs unpack a
 // stage in 1300 clocks and hold its slot meanwhile.  What was tried: the products issued by a thread that also unpacks (twice the time), by a thread chosen by its number instead of
 // elect.sync (41 us for 64 rows, 31 now), sums back of one stage of fp32 rows (7e-7 off instead of 1.1e-6, 5 % slower), eight warps that both unpack and sum (528 us for 4096 rows, 319 now).
@@ -40,7 +40,7 @@ constexpr int A_BYTES = LANES * STEP * 2;
 // Warps: eight that sum, pairs that unpack a stage each in turn, one that copies, one that issues.  Launched with 128 registers a thread; the eight take 168 (they hold up
 // to 128 sums), for which the others give up all but 80: 256 * 168 + 256 * 80 is within 512 * 128.
 constexpr int SUMMERS = 8, TEAM = 64, COPIER = 14, ISSUER = 15, THREADS = 512;
-__host__ __device__ constexpr int back_stages(int weight_parts) { return weight_parts == 3 ? 2 : 8; }  // of a sum of a W: 48 MMA steps (six products of parts), or 64 to 96 beside a result of 16 bits
+__host__ __device__ constexpr int back_stages(int weight_parts) { return weight_parts == 3 ? 2 : 8; }  // of a sum of a W: 48 MMA steps (six products of parts), or 64 to 128 beside a result of 16 bits
 constexpr int HEADER = 1024;          // of the workspace: the status word, then a bit for each tile of rows and 64 summed indices that hold a number that is not finite
 constexpr int RING = 224 * 1024;
 
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
                   if (!ok) break;
                   b = b_first + (uint64_t)(slot * (B_BYTES >> 4));
                 }
-                if (FORWARD || q + part < WP) mma_step<SLICE>(d, a + (uint64_t)(q * (A_BYTES >> 4)), b, idesc, !(anew && part == 0 && q == 0));
+                if (FORWARD || WP == 2 || q + part < WP) mma_step<SLICE>(d, a + (uint64_t)(q * (A_BYTES >> 4)), b, idesc, !(anew && part == 0 && q == 0));
               }
               if (!ok) break;
               mma_commit(smem_u32(&ctl->b_empty[slot]));
@@ -477,7 +477,6 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
           for (int r = 0; r < 4; ++r) {
             const uint32_t word[4] = {codes[b][r].x, codes[b][r].y, codes[b][r].z, codes[b][r].w};
             const float f = FORWARD ? 1.f : absolute ? fabsf(scale[b][r]) : scale[b][r];
-            const __nv_bfloat162 f1 = __float2bfloat162_rn(f), f2 = __float2bfloat162_rn(f - __low2float(f1));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t at = to + (r >> 1) * 8192 + (((uint32_t)((r & 1) * 4 + e) ^ (uint32_t)(t & 7)) << 4);
@@ -493,12 +492,12 @@ __global__ void __launch_bounds__(THREADS, 1) w4_many_kernel(const ManyArgs p) {
                 uint32_t part[WP][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  if (WP == 2) {  // the first part of code times the scale's first part, the rest of that product (exact), and the code times the scale's second part
-                  const __nv_bfloat162 c = *reinterpret_cast<const __nv_bfloat162*>(&q[i]), high = __hmul2(c, f1);
-                  part[0][i] = bits_of(high);
-                  part[WP - 1][i] = bits_of(__hfma2(c, f2, __hfma2(c, f1, __hneg2(high))));
-                  continue;
-                }
+                  if (WP == 2) {  // the product rounded to the nearest, and what that leaves of it
+                    const float c0 = __uint_as_float(q[i] << 16), c1 = __uint_as_float(q[i] & 0xffff0000u);
+                    part[0][i] = bits_of(__floats2bfloat162_rn(c0 * f, c1 * f));
+                    part[WP - 1][i] = bits_of(__floats2bfloat162_rn(fmaf(c0, f, -__uint_as_float(part[0][i] << 16)), fmaf(c1, f, -__uint_as_float(part[0][i] & 0xffff0000u))));
+                    continue;
+                  }
                   float x = __uint_as_float(q[i] << 16) * f, y = __uint_as_float(q[i] & 0xffff0000u) * f;
 #pragma unroll
                   for (int k = 0; k < WP; ++k) {

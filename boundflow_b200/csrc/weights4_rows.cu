@@ -342,7 +342,7 @@ int backward(const W4RowsArgs& p, Split sp, int tiles_m, cudaStream_t stream) {
 
 int launch_w4_rows(const W4RowsArgs& all, cudaStream_t stream) {
   Split sp = {};
-  const int parts = all.type == BF_TYPE_F32 ? 3 : 2;  // a 16-bit row times a 32-bit scale: two parts hold it to 2^-18
+  const int parts = all.type == BF_TYPE_F32 ? 3 : 2;  // a 16-bit row times a 32-bit scale: two parts hold it to 2^-17
   const bool dual = all.b != nullptr;
   sp.packed = all.M * parts <= 8;
   const int nt = dual || sp.packed || all.M <= 8 ? 1 : 2;
